@@ -145,7 +145,21 @@ def _tables(c, g, lens):
 
 
 def prepare(case, seed):
-    c = case
+    s = _inputs(case, seed)
+    if own:                          # what a program keeps: its layer's cache, its model's table, a step's work list
+        from enterprise_inference_amd.ops import quant_cache as Q
+        from enterprise_inference_amd.ops.rotary import RotaryCache
+        c = case
+        s["cache"] = Q.QuantKVCache(s["k"], s["v"], s["k_scale"], s["v_scale"])
+        if c["op"] == "append":
+            s["rotary"] = RotaryCache.from_table(s["cos_sin"])
+        if c["op"] == "chunk":
+            s["plan"] = Q.quant_prefill_plan(*_lens(c), c["heads"], c["kv_heads"], c["dim"], "cuda", causal=c["causal"],
+                                             sliding_window=c["window"] or None)
+    return s
+
+
+def _inputs(c, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     h, hk, d, bs = c["heads"], c["kv_heads"], c["dim"], c["page"]
     s = dict(case=c)
@@ -179,9 +193,6 @@ def prepare(case, seed):
         for n in new:
             cu.append(cu[-1] + n)
         s["cu_q"], s["most"] = _i32(cu), max(new)
-        if own:                      # the step's work list, which a program keeps for all of its layers
-            from enterprise_inference_amd.ops import quant_cache as Q
-            s["plan"] = Q.quant_prefill_plan(new, lens, h, hk, d, "cuda", causal=c["causal"], sliding_window=c["window"] or None)
     return s
 
 
@@ -272,11 +283,10 @@ def run(state):
     if not own:
         return {"append": _append, "read": _read, "decode": _decode, "chunk": _chunk}[c["op"]](s)
     from enterprise_inference_amd.ops import quant_cache as Q
-    from enterprise_inference_amd.ops.rotary import RotaryCache
-    cache = Q.QuantKVCache(s["k"], s["v"], s["k_scale"], s["v_scale"])
+    cache = s["cache"]
     if c["op"] == "append":
-        q = Q.rope_qkv_quant(s["qkv"], s["positions"], RotaryCache.from_table(s["cos_sin"]), s["slots"], cache, c["heads"],
-                             c["kv_heads"], c["dim"], bias=s["bias"], q_norm_w=s["q_norm"], k_norm_w=s["k_norm"], norm_eps=1e-6)
+        q = Q.rope_qkv_quant(s["qkv"], s["positions"], s["rotary"], s["slots"], cache, c["heads"], c["kv_heads"], c["dim"],
+                             bias=s["bias"], q_norm_w=s["q_norm"], k_norm_w=s["k_norm"], norm_eps=1e-6)
         return (q, *Q.quant_read(cache, s["slots"]))
     if c["op"] == "read":
         return Q.quant_read(cache, s["slots"])
