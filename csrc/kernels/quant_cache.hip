@@ -1,0 +1,302 @@
+// Writing and reading the 8-bit key/value cache (eia_quant.h).
+//
+// The write takes the QKV projection's rows [T, (Hq + 2 Hkv) D] (bf16, or the fp32 partial sums of a split-K GEMM):
+// bias, RMS norm of queries and keys, rotation; queries go on in bf16, keys and values into the cache.  All of it in
+// fp32, rounded once: a key's code is the nearest to the rotated fp32 value.
+//
+// A head of a token is D / 16 lanes, sixteen values a lane (two halves of eight, as they rotate); the lanes of a kv head
+// hold the key row and the value row, because a value that is not finite marks both.  A workgroup takes TT tokens and
+// 64 / (D / 16) query heads, or as many kv heads as fill it.  Codes of values go through LDS so that sixteen tokens of a
+// channel are stored together where their slots are (a prompt's are, but for its first and last group).
+#include "eia_quant.h"
+
+namespace {
+
+struct QuantSrc {
+  const bf16_t* qkv;       // [T][stride], or
+  const float* part;       // split-K sums [sk][T][(Hq + 2 Hkv) D]
+  long stride, slab;
+  int sk;
+  const bf16_t *bias, *q_norm, *k_norm;
+  float eps;
+};
+
+template <int D, bool NEOX> EIA_DEV void halves_of(int sub, int& e0, int& e1) {
+  e0 = NEOX ? 8 * sub : 16 * sub;
+  e1 = NEOX ? D / 2 + 8 * sub : 16 * sub + 8;
+}
+
+// Sixteen values of a head's row, with the bias.
+template <int D, bool NEOX>
+EIA_DEV void load_row(const QuantSrc& src, int t, int head, int ntot, int sub, float (&x)[16]) {
+  int e[2];
+  halves_of<D, NEOX>(sub, e[0], e[1]);
+  if (src.part) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = 0.f;
+    for (int k = 0; k < src.sk; ++k) {
+      const float* p = src.part + k * src.slab + ((long)t * ntot + head) * D;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(p + e[h] + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[8 * h + 4 * q + j] += v[j];
+        }
+    }
+  } else {
+    const bf16_t* p = src.qkv + (long)t * src.stride + (long)head * D;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x8 v = *reinterpret_cast<const bf16x8*>(p + e[h]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[8 * h + j] = bf2f(v[j]);
+    }
+  }
+  if (src.bias) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x8 v = *reinterpret_cast<const bf16x8*>(src.bias + (long)head * D + e[h]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[8 * h + j] += bf2f(v[j]);
+    }
+  }
+}
+
+template <int D, bool NEOX>
+EIA_DEV void norm_row(const bf16_t* w, float eps, int sub, float (&x)[16]) {
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) ss += x[j] * x[j];
+#pragma unroll
+  for (int o = 1; o < D / 16; o <<= 1) ss += __shfl_xor(ss, o, 64);
+  const float inv = 1.f / sqrtf(ss / (float)D + eps);
+  int e[2];
+  halves_of<D, NEOX>(sub, e[0], e[1]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(w + e[h]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[8 * h + j] *= inv * bf2f(v[j]);
+  }
+}
+
+// cs: cos [D / 2] | sin [D / 2] of the token's position.
+template <int D, bool NEOX>
+EIA_DEV void rotate_row(const float* cs, int sub, float (&x)[16]) {
+  float c[8], s[8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(cs + 8 * sub + 4 * q), b = *reinterpret_cast<const f32x4*>(cs + D / 2 + 8 * sub + 4 * q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[4 * q + j] = a[j], s[4 * q + j] = b[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float &a = x[NEOX ? j : 2 * j], &b = x[NEOX ? 8 + j : 2 * j + 1];
+    const float ra = fmaf(a, c[j], -(b * s[j])), rb = fmaf(b, c[j], a * s[j]);
+    a = ra;
+    b = rb;
+  }
+}
+
+template <int D, bool NEOX, int TT>
+__global__ void __launch_bounds__(256)
+quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float* __restrict__ cos_sin,
+                   const int* __restrict__ slots, QuantCache cache, long num_slots, bf16_t* __restrict__ q_out, int T, int Hq,
+                   int q_groups) {
+  constexpr int TPH = D / 16, HPB = 256 / TPH / TT;        // lanes of a head, heads of a workgroup
+  static_assert(HPB >= 1, "");
+  const int sub = threadIdx.x % TPH, at = threadIdx.x / TPH;
+  const int i = at % TT, t = blockIdx.x * TT + i, Hkv = cache.Hkv, ntot = Hq + 2 * Hkv;
+  int e0, e1;
+  halves_of<D, NEOX>(sub, e0, e1);
+  if ((int)blockIdx.y < q_groups) {
+    const int h = blockIdx.y * HPB + at / TT;
+    if (t >= T || h >= Hq) return;                         // (a head's lanes together)
+    float x[16];
+    load_row<D, NEOX>(src, t, h, ntot, sub, x);
+    if (src.q_norm) norm_row<D, NEOX>(src.q_norm, src.eps, sub, x);
+    if (cos_sin) rotate_row<D, NEOX>(cos_sin + (long)positions[t] * D, sub, x);
+    bf16x8 a, b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = f2bf(x[j]), b[j] = f2bf(x[8 + j]);
+    bf16_t* o = q_out + ((long)t * Hq + h) * D;
+    *reinterpret_cast<bf16x8*>(o + e0) = a;
+    *reinterpret_cast<bf16x8*>(o + e1) = b;
+    return;
+  }
+  __shared__ __align__(16) uint8_t tile[HPB][D][TT];
+  const int hh = at / TT, h = (blockIdx.y - q_groups) * HPB + hh;
+  const long slot = t < T ? slots[t] : -1;
+  const bool live = slot >= 0 && slot < num_slots && h < Hkv;
+  if (live) {
+    float k[16], v[16];
+    load_row<D, NEOX>(src, t, Hq + h, ntot, sub, k);
+    load_row<D, NEOX>(src, t, Hq + Hkv + h, ntot, sub, v);
+    if (src.k_norm) norm_row<D, NEOX>(src.k_norm, src.eps, sub, k);
+    if (cos_sin) rotate_row<D, NEOX>(cos_sin + (long)positions[t] * D, sub, k);
+    // magnitudes as bits: what is not finite is the largest
+    unsigned mk = 0, mv = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      mk = max(mk, __float_as_uint(k[j]) & 0x7fffffffu);
+      mv = max(mv, __float_as_uint(v[j]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = 1; o < TPH; o <<= 1) {
+      mk = max(mk, (unsigned)__shfl_xor((int)mk, o, 64));
+      mv = max(mv, (unsigned)__shfl_xor((int)mv, o, 64));
+    }
+    const bool poison = max(mk, mv) >= 0x7f800000u;
+    const unsigned bk = poison ? QUANT_POISON : quant_byte(mk), bv = poison ? 127 : quant_byte(mv);
+    const int page = (int)(slot / cache.bs), off = (int)(slot % cache.bs);
+    unsigned w[4], u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = poison ? 0 : quant_pack(k[4 * j], k[4 * j + 1], k[4 * j + 2], k[4 * j + 3], quant_inverse(bk));
+      u[j] = poison ? 0 : quant_pack(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], quant_inverse(bv));
+    }
+    uint8_t* kp = cache.key(page, h, off, D);
+    *reinterpret_cast<uint2*>(kp + e0) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(kp + e1) = make_uint2(w[2], w[3]);
+    if (sub == 0) {
+      *cache.kscale(page, h, off) = (uint8_t)bk;
+      *cache.vscale(page, h, off) = (uint8_t)bv;
+    }
+    if constexpr (TT == QUANT_GROUP) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) tile[hh][j < 8 ? e0 + j : e1 + j - 8][i] = (uint8_t)(u[j / 4] >> (8 * (j & 3)));
+    } else {
+      uint8_t* vp = cache.values(page, h, off & ~(QUANT_GROUP - 1), D) + off % QUANT_GROUP;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) vp[QUANT_GROUP * (j < 8 ? e0 + j : e1 + j - 8)] = (uint8_t)(u[j / 4] >> (8 * (j & 3)));
+    }
+  }
+  if constexpr (TT == QUANT_GROUP) {
+    __syncthreads();
+    // whole groups: their first slot is a multiple of 16 and the others follow (the same for the whole workgroup)
+    const int t0 = blockIdx.x * TT, lane = threadIdx.x & 15;
+    const int mine = t0 + lane < T ? slots[t0 + lane] : -1, first = slots[t0];
+    const bool whole = __all(mine == first + lane) && first >= 0 && first % QUANT_GROUP == 0 && (long)first + QUANT_GROUP <= num_slots;
+    if (whole) {
+      const int page = first / cache.bs, off = first % cache.bs;
+      for (int r = threadIdx.x; r < HPB * D; r += 256) {
+        const int g = (blockIdx.y - q_groups) * HPB + r / D;
+        if (g < Hkv) *reinterpret_cast<uint4*>(cache.values(page, g, off, D) + QUANT_GROUP * (r % D)) = *reinterpret_cast<const uint4*>(&tile[r / D][r % D][0]);
+      }
+    } else {
+      const bool there = mine >= 0 && mine < num_slots;
+      const int page = there ? mine / cache.bs : 0, off = there ? mine % cache.bs : 0;
+      for (int r = threadIdx.x / 16; r < HPB * D; r += 16) {
+        const int g = (blockIdx.y - q_groups) * HPB + r / D;
+        if (g < Hkv && there) cache.values(page, g, off & ~(QUANT_GROUP - 1), D)[QUANT_GROUP * (r % D) + off % QUANT_GROUP] = tile[r / D][r % D][lane];
+      }
+    }
+  }
+}
+
+// Rows of sixteen slots and one head a workgroup part: keys straight through, values through LDS as the cache holds them.
+// Rows of slots outside the cache are zeros.
+template <int D>
+__global__ void __launch_bounds__(256)
+quant_read_kernel(QuantCache cache, const int* __restrict__ slots, long num_slots, int n, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out) {
+  constexpr int TPH = D / 16, HPB = 256 / TPH / QUANT_GROUP;
+  __shared__ __align__(16) uint8_t tile[HPB][D * QUANT_GROUP];
+  const int t0 = blockIdx.x * QUANT_GROUP, Hkv = cache.Hkv, h0 = blockIdx.y * HPB;
+  const int lane = threadIdx.x & 15;
+  const int mine = t0 + lane < n ? slots[t0 + lane] : -1, first = slots[t0];
+  const bool whole = __all(mine == first + lane) && first >= 0 && first % QUANT_GROUP == 0 && (long)first + QUANT_GROUP <= num_slots;
+  const bool there = mine >= 0 && mine < num_slots;
+  if (whole) {
+    const int page = first / cache.bs, off = first % cache.bs;
+    for (int r = threadIdx.x; r < HPB * D; r += 256)
+      if (h0 + r / D < Hkv)
+        *reinterpret_cast<uint4*>(&tile[r / D][QUANT_GROUP * (r % D)]) = *reinterpret_cast<const uint4*>(cache.values(page, h0 + r / D, off, D) + QUANT_GROUP * (r % D));
+  } else {
+    const int page = there ? mine / cache.bs : 0, off = there ? mine % cache.bs : 0;
+    for (int r = threadIdx.x / 16; r < HPB * D; r += 16)
+      if (h0 + r / D < Hkv)
+        tile[r / D][QUANT_GROUP * (r % D) + lane] = there ? cache.values(page, h0 + r / D, off & ~(QUANT_GROUP - 1), D)[QUANT_GROUP * (r % D) + off % QUANT_GROUP] : 0;
+  }
+  __syncthreads();
+  const int sub = threadIdx.x % TPH, i = threadIdx.x / TPH % QUANT_GROUP, hh = threadIdx.x / TPH / QUANT_GROUP, h = h0 + hh, t = t0 + i;
+  if (t >= n || h >= Hkv) return;
+  const long slot = slots[t];
+  const bool live = slot >= 0 && slot < num_slots;
+  const int page = live ? (int)(slot / cache.bs) : 0, off = live ? (int)(slot % cache.bs) : 0;
+  const unsigned bk = live ? *cache.kscale(page, h, off) : 127, bv = live ? *cache.vscale(page, h, off) : 127;
+  uint4 w = live ? *reinterpret_cast<const uint4*>(cache.key(page, h, off, D) + 16 * sub) : make_uint4(0, 0, 0, 0), u;
+  unsigned x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) x[j] |= (unsigned)tile[hh][QUANT_GROUP * (16 * sub + 4 * j + b) + i] << (8 * b);
+  }
+  u = make_uint4(x[0], x[1], x[2], x[3]);
+  if (bk == QUANT_POISON) w = u = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+  const float sk = bk == QUANT_POISON ? 1.f : quant_scale(bk), sv = quant_scale(bv);
+  const long o = ((long)t * Hkv + h) * D + 16 * sub;
+  *reinterpret_cast<bf16x8*>(k_out + o) = quant_eight(w.x, w.y, sk);
+  *reinterpret_cast<bf16x8*>(k_out + o + 8) = quant_eight(w.z, w.w, sk);
+  *reinterpret_cast<bf16x8*>(v_out + o) = quant_eight(u.x, u.y, sv);
+  *reinterpret_cast<bf16x8*>(v_out + o + 8) = quant_eight(u.z, u.w, sv);
+}
+
+}  // namespace
+
+// qkv bf16 rows, or part != nullptr: fp32 sums [sk][T][(Hq + 2 Hkv) D].  cos_sin nullptr: no rotation.
+EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part, int sk, const int* positions, const float* cos_sin,
+                            const int* slots, void* k, void* v, void* ks, void* vs, long codes, long scales, int pages, void* q_out,
+                            const void* bias, const void* q_norm, const void* k_norm, float eps, int T, int Hq, int Hkv, int D, int bs,
+                            int neox, hipStream_t st) {
+  if (T < 0 || Hq <= 0 || Hkv <= 0 || bs <= 0 || bs % QUANT_GROUP || (part && sk < 1) || (!q_norm) != (!k_norm)) return EIA_BAD_SHAPE;
+  if (T == 0) return EIA_OK;
+  const QuantSrc src{(const bf16_t*)qkv, part, qkv_stride, (long)T * (Hq + 2 * Hkv) * D, sk, (const bf16_t*)bias, (const bf16_t*)q_norm,
+                     (const bf16_t*)k_norm, eps};
+  const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
+#define QW_GO(D, NX, TT)                                                                                                          \
+  do {                                                                                                                            \
+    constexpr int hpb = 256 / (D / 16) / TT;                                                                                      \
+    const int qg = (Hq + hpb - 1) / hpb;                                                                                          \
+    hipLaunchKernelGGL((quant_write_kernel<D, NX, TT>), dim3((T + TT - 1) / TT, qg + (Hkv + hpb - 1) / hpb), dim3(256), 0, st, src, \
+                       positions, cos_sin, slots, c, (long)pages * bs, (bf16_t*)q_out, T, Hq, qg);                                \
+  } while (0)
+#define QW_D(D)                                                                                          \
+  do {                                                                                                   \
+    if (T >= 256) { if (neox) QW_GO(D, true, 16); else QW_GO(D, false, 16); }                            \
+    else { if (neox) QW_GO(D, true, 1); else QW_GO(D, false, 1); }                                       \
+  } while (0)
+  switch (D) {
+    case 64: QW_D(64); break;
+    case 128: QW_D(128); break;
+    case 256: QW_D(256); break;
+    default: return EIA_UNSUPPORTED;
+  }
+#undef QW_D
+#undef QW_GO
+  EIA_LAUNCH_CHECK();
+}
+
+EIA_API int eia_quant_read(const void* k, const void* v, const void* ks, const void* vs, long codes, long scales, int pages,
+                           const int* slots, int n, void* k_out, void* v_out, int Hkv, int D, int bs, hipStream_t st) {
+  if (n < 0 || Hkv <= 0 || bs <= 0 || bs % QUANT_GROUP) return EIA_BAD_SHAPE;
+  if (n == 0) return EIA_OK;
+  const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
+#define QR_GO(D)                                                                                                                   \
+  do {                                                                                                                             \
+    constexpr int hpb = 256 / (D / 16) / QUANT_GROUP;                                                                              \
+    hipLaunchKernelGGL(quant_read_kernel<D>, dim3((n + QUANT_GROUP - 1) / QUANT_GROUP, (Hkv + hpb - 1) / hpb), dim3(256), 0, st, c, \
+                       slots, (long)pages * bs, n, (bf16_t*)k_out, (bf16_t*)v_out);                                                \
+  } while (0)
+  switch (D) {
+    case 64: QR_GO(64); break;
+    case 128: QR_GO(128); break;
+    case 256: QR_GO(256); break;
+    default: return EIA_UNSUPPORTED;
+  }
+#undef QR_GO
+  EIA_LAUNCH_CHECK();
+}

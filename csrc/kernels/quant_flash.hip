@@ -1,0 +1,404 @@
+// Attention of chunks of new tokens over the 8-bit cache (eia_quant.h), on v_mfma_f32_32x32x16_bf16.
+//
+// The queries of a sequence and the G heads of a kv head make rows (query, head), query first; a workgroup takes a block
+// of them, 32 a wave, so that a tile of 64 keys and values is fetched once for the block whatever G is.  A wave holds its
+// rows as columns: S^T[key, row] = K Q^T, then O^T[channel, row] += V^T P^T with P^T taken from the S^T accumulators as
+// they lie (K rows enter with bits 2 and 3 of their number exchanged, so that an accumulator's elements are eight keys in
+// a row).  A lane owns one row together with lane ^ 32.
+//
+// A tile comes from memory as codes, half the bytes of bf16, and is converted once on its way into LDS: a key's scale is
+// the conversion's; values lie as sixteen tokens of a channel, whose scales differ, so each pair is converted twice and
+// the halves are put together (24 instructions for 16 values).  Both are exact; the products run as with a bf16 cache.
+//
+// The host lays the launch out (which rows, which tiles): blocks that would be the launch's tail are cut along the keys,
+// their parts hand over fp32 sums and a second kernel puts them together.
+#include "eia_flash.h"
+#include "eia_quant.h"
+
+namespace {
+
+constexpr int FK = 64;               // keys of a tile
+
+template <int D> struct Shape {
+  static constexpr int THREADS = D == 256 ? 256 : 512;    // 256 channels: four waves, one a SIMD (320 registers)
+  static constexpr int ROWS = THREADS / 64 * 32;
+  static constexpr int KS = D + 8, VS = FK + 8;           // row strides in LDS: 16 bytes apart from a power of two
+  static constexpr int BUF = FK * KS + D * VS;
+};
+
+struct Item { int seq, row, lo, tiles, slot, pad[3]; };    // row block, first key, key tiles, place of a part's sums (-1: whole)
+struct Merge { int seq, row, slot, parts; };
+
+struct Chunk {
+  const bf16_t* q;
+  bf16_t* out;
+  long q_stride, out_stride;
+  const int *tables, *lens, *cu;
+  int bt_stride, Hq, causal, window, chunk;
+  float scale_log2;
+  f32x4* po;                         // sums of a part as its lanes hold them [slot][kv head][wave][D / 8][64]
+  float2* ml;                        // [slot][kv head][wave][32]
+  int groups;
+  unsigned magic;
+};
+
+EIA_DEV int swap_bits(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
+
+EIA_DEV int first_key(int qa, int window, int chunk) {
+  int lo = 0;
+  if (window > 0) lo = max(lo, qa - window + 1);
+  if (chunk > 0 && qa > 0) lo = max(lo, qa / chunk * chunk);
+  return lo;
+}
+
+// 32 channels of a row: lane half h holds channels 8 j + 4 h .. + 3; halves of pairs change places, for 16-byte stores.
+EIA_DEV void put_row(bf16_t* op, const f32x16_t& o, float inv) {
+  uint2 pk[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    pk[j] = make_uint2(__builtin_bit_cast(unsigned, flash_pack(o[4 * j] * inv, o[4 * j + 1] * inv)),
+                       __builtin_bit_cast(unsigned, flash_pack(o[4 * j + 2] * inv, o[4 * j + 3] * inv)));
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const auto x = __builtin_amdgcn_permlane32_swap(pk[j].x, pk[j + 1].x, false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(pk[j].y, pk[j + 1].y, false, false);
+    *reinterpret_cast<uint4*>(op + 8 * j) = make_uint4(x[0], y[0], x[1], y[1]);
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(Shape<D>::THREADS, 1)
+quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
+  constexpr int NT = Shape<D>::THREADS, KS = Shape<D>::KS, VS = Shape<D>::VS, BUF = Shape<D>::BUF;
+  constexpr int PIECES = 4 * D;                            // 16-byte pieces of a tile's keys, and of its values
+  constexpr bool SHARED = PIECES < NT;                     // half the threads take keys, half values
+  constexpr int NP = SHARED ? 1 : PIECES / NT;
+  static_assert(!SHARED || 2 * PIECES == NT, "");
+  __shared__ __align__(16) bf16_t lds[2 * BUF];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r32 = lane & 31, h = lane >> 5;
+  const Item it = items[blockIdx.y];
+  const int kvh = blockIdx.x, Hkv = cache.Hkv, G = a.Hq / Hkv;
+  const int qbeg = a.cu[it.seq], qlen = a.cu[it.seq + 1] - qbeg, L = a.lens[it.seq], ctx = L - qlen;
+  const int rows = qlen * G, row0 = it.row + 32 * w;
+  const bool window = a.window > 0 || a.chunk > 0;
+  const int row = min(row0 + r32, rows - 1), qi = row / G;
+  const long tok = qbeg + qi;
+  const int hq = kvh * G + row - qi * G;
+  const int qa = ctx + qi, q_lo = first_key(qa, a.window, a.chunk);
+  const int kmax = a.causal ? min(L - 1, qa) : L - 1;
+
+  bf16x8 qf[D / 16];                                       // step t: channels 16 t + 8 h .. + 7
+  {
+    const bf16_t* qp = a.q + tok * a.q_stride + (long)hq * D + 8 * h;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(qp + 16 * t);
+  }
+  const bool live = row0 < rows;
+  const int wq0 = min(row0, rows - 1) / G, wq1 = min(row0 + 31, rows - 1) / G;     // the wave's first and last query
+  const int w_hi = !live ? 0 : a.causal ? min(L, ctx + wq1 + 1) : L;
+  const int w_lo = first_key(ctx + wq0, a.window, a.chunk);
+
+  const int* bt = a.tables + (long)it.seq * a.bt_stride;
+  const int last = max(L - 1, 0) / QUANT_GROUP;
+  const bool keys_here = !SHARED || tid < PIECES, values_here = !SHARED || tid >= PIECES;
+  auto piece = [&](int i) { return SHARED ? tid % PIECES : tid + NT * i; };
+  // a wave's pieces of keys and of values lie in one group of 16 tokens, the same for both
+  int page[NP], off[NP];
+  auto look = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int group = __builtin_amdgcn_readfirstlane(min((it.lo + FK * tile) / QUANT_GROUP + piece(i) / D, last));
+      const int at = a.groups == 1 ? group : (int)__umulhi((unsigned)group, a.magic);
+      page[i] = bt[at];
+      off[i] = QUANT_GROUP * (a.groups == 1 ? 0 : group - at * a.groups);
+    }
+  };
+  uint4 kst[NP], vst[NP], vsc[NP];
+  unsigned ksc[NP];
+  auto fetch = [&] {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int pg = __builtin_amdgcn_readfirstlane(page[i]), id = piece(i);
+      if (keys_here) {
+        const int r = id / (D / 16) % QUANT_GROUP;
+        kst[i] = *reinterpret_cast<const uint4*>(cache.key(pg, kvh, off[i] + r, D) + 16 * (id % (D / 16)));
+        ksc[i] = *cache.kscale(pg, kvh, off[i] + r);
+      }
+      if (values_here) {
+        vst[i] = *reinterpret_cast<const uint4*>(cache.values(pg, kvh, off[i], D) + 16 * (id % D));
+        vsc[i] = *reinterpret_cast<const uint4*>(cache.vscale(pg, kvh, off[i]));
+      }
+    }
+  };
+  auto stash = [&](int buf, int tile) {
+    bf16_t* kl = lds + buf * BUF;
+    bf16_t* vl = kl + FK * KS;
+    const int kb = it.lo + FK * tile;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int id = piece(i);
+      if (keys_here) {
+        uint4 x = kst[i];
+        const bool poison = ksc[i] == QUANT_POISON;        // a token that is no number
+        if (poison) x = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+        const float sc = quant_scale(poison ? 127 : ksc[i]);
+        bf16_t* p = kl + id / (D / 16) * KS + 16 * (id % (D / 16));
+        *reinterpret_cast<bf16x8*>(p) = quant_eight(x.x, x.y, sc);
+        *reinterpret_cast<bf16x8*>(p + 8) = quant_eight(x.z, x.w, sc);
+      }
+      if (values_here) {
+        uint4 x = vst[i];
+        unsigned sb[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sb[j] = __builtin_amdgcn_readfirstlane((&vsc[i].x)[j]);
+        const int group = __builtin_amdgcn_readfirstlane(id / D);
+        if (kb + QUANT_GROUP * (group + 1) > L) {          // keys past the end: whatever lies there, nothing of it is kept
+          const int n = max(L - kb - QUANT_GROUP * group, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = min(max(n - 4 * j, 0), 4);
+            const unsigned keep = k == 4 ? ~0u : (1u << (8 * k)) - 1;
+            (&x.x)[j] &= keep;
+            sb[j] &= keep;
+          }
+        }
+        bf16_t* p = vl + id % D * VS + QUANT_GROUP * group;
+        unsigned y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned word = (&x.x)[j];
+          float s[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) s[b] = quant_scale((sb[j] >> (8 * b)) & 255u);
+          y[2 * j] = (quant_pair<false>(word, s[0]) & 0xffffu) | (quant_pair<false>(word, s[1]) & 0xffff0000u);
+          y[2 * j + 1] = (quant_pair<true>(word, s[2]) & 0xffffu) | (quant_pair<true>(word, s[3]) & 0xffff0000u);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(p + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+    }
+  };
+
+  f32x16_t o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const int krow = swap_bits(r32);
+
+  auto compute = [&](int buf, int kb) {
+    const bf16_t* kf0 = lds + buf * BUF + krow * KS + 8 * h;
+    const bf16_t* vf0 = lds + buf * BUF + FK * KS + r32 * VS + 8 * h;
+    f32x16_t sc[2];
+    // reads of LDS go four fragments ahead of the products; products go before the other wave's vector work
+    bf16x8 kf[2][4];
+    auto keys = [&](int b) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) kf[b & 1][x] = *reinterpret_cast<const bf16x8*>(kf0 + 32 * KS * (x & 1) + 16 * (2 * b + (x >> 1)));
+    };
+    __builtin_amdgcn_s_setprio(1);
+    keys(0);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) {
+      if (b + 1 < D / 32) keys(b + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = 2 * b + (x >> 1);
+        sc[x & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b & 1][x], qf[t], t == 0 ? f32x16_t{} : sc[x & 1], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    // element i of half sh is key kb + 32 sh + 16 (i / 8) + 8 h + i % 8
+    const bool whole = !window && kb + FK <= L && (!a.causal || kb + FK - 1 <= ctx + wq0);
+    mfma_settle(sc[0], sc[1]);
+    if (!whole) {
+      // seen: q_lo <= key <= kmax, as one unsigned comparison (a row that sees nothing compares with a far place)
+      const unsigned lim = kmax >= q_lo ? (unsigned)(kmax - q_lo) : 0u;
+      const int d0 = kmax >= q_lo ? kb + 8 * h - q_lo : 1 << 30;
+#pragma unroll
+      for (int sh = 0; sh < 2; ++sh)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[sh][i] = (unsigned)(d0 + 32 * sh + 16 * (i >> 3) + (i & 7)) <= lim ? sc[sh][i] : -INFINITY;
+    }
+    float mx4[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      mx4[c] = sc[c >> 1][8 * (c & 1)];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx4[c] = fmaxf(mx4[c], sc[c >> 1][8 * (c & 1) + j]);
+    }
+    const float mt = flash_pair_max(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]))) * a.scale_log2;
+    // the running maximum moves only where a tile exceeds it by more than 2^8: weights stay below 256, sums in fp32
+    const bool grow = mt > m + FLASH_DEFER;
+    if (__any(grow)) {
+      const float now = grow ? mt : m, old = grow ? exp2f(m - now) : 1.f;
+      m = now;
+      l *= old;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] *= old;
+    }
+    const float use = m == -INFINITY ? 0.f : m;
+    bf16x8 p[4];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    auto weights = [&](int ks) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(sc[ks >> 1][8 * (ks & 1) + j], a.scale_log2, -use));
+        p[ks][j] = f2bf(e);
+        sum[ks] += e;
+      }
+    };
+    constexpr int VB = D / 32 < 4 ? D / 32 : 4;            // fragments of values read ahead
+    bf16x8 vf[2][VB];
+    auto values = [&](int s) {                             // step s: channels of block s % (D / 32 / VB), keys of s / (...)
+      constexpr int NB = D / 32 / VB;
+#pragma unroll
+      for (int x = 0; x < VB; ++x) vf[s & 1][x] = *reinterpret_cast<const bf16x8*>(vf0 + 32 * VS * (VB * (s % NB) + x) + 16 * (s / NB));
+    };
+    __builtin_amdgcn_s_setprio(2);
+    values(0);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(0);
+    constexpr int NB = D / 32 / VB;
+#pragma unroll
+    for (int s = 0; s < 4 * NB; ++s) {
+      if (s + 1 < 4 * NB) {
+        values(s + 1);
+        if ((s + 1) % NB == 0) weights((s + 1) / NB);
+      }
+#pragma unroll
+      for (int x = 0; x < VB; ++x)
+        o[VB * (s % NB) + x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s & 1][x], p[s / NB], o[VB * (s % NB) + x], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  if (it.tiles > 0) {
+    look(0);
+    fetch();
+    if (it.tiles > 1) look(1);
+    stash(0, 0);
+  }
+  __syncthreads();
+  for (int t = 0; t < it.tiles; ++t) {
+    const int kb = it.lo + FK * t;
+    const bool more = t + 1 < it.tiles;
+    if (more) {
+      fetch();
+      if (t + 2 < it.tiles) look(t + 2);
+    }
+    if (kb < w_hi && kb + FK > w_lo) compute(t & 1, kb);   // (the same for the wave)
+    if (more) stash((t + 1) & 1, t + 1);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) mfma_settle(o[dt]);
+  const float lt = flash_pair_sum(l);
+  if (it.slot >= 0) {
+    if (!live) return;
+    const long at = ((long)it.slot * Hkv + kvh) * (NT / 64) + w;
+    f32x4* po = a.po + at * (D / 8 * 64) + lane;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) po[(4 * dt + j) * 64] = f32x4{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+    if (h == 0) a.ml[at * 32 + r32] = make_float2(m, lt);
+    return;
+  }
+  if (row0 + r32 >= rows) return;
+  const float inv = lt != 0.f ? 1.f / lt : 0.f;
+  bf16_t* op = a.out + tok * a.out_stride + (long)hq * D + 8 * h;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) put_row(op + 32 * dt, o[dt], inv);
+}
+
+// A workgroup puts the parts of one wave's 32 rows together, a wave 32 channels at a time.
+template <int D>
+__global__ void __launch_bounds__(256)
+quant_flash_merge_kernel(Chunk a, int Hkv, const Merge* __restrict__ merges) {
+  constexpr int W = Shape<D>::THREADS / 64;
+  const Merge it = merges[blockIdx.z];
+  const int kvh = blockIdx.x, w = blockIdx.y, lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, G = a.Hq / Hkv;
+  const int qbeg = a.cu[it.seq], rows = (a.cu[it.seq + 1] - qbeg) * G, row0 = it.row + 32 * w;
+  if (row0 >= rows) return;
+  const long step = (long)Hkv * W, at = ((long)it.slot * Hkv + kvh) * W + w;
+  const float2* ml = a.ml + at * 32 + r32;
+  for (int dt = threadIdx.x >> 6; dt < D / 32; dt += 4) {
+    const f32x4* po = a.po + at * (D / 8 * 64) + dt * 4 * 64 + lane;
+    f32x16_t o;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (int p0 = 0; p0 < it.parts; p0 += 4) {
+      float2 x[4];
+      f32x4 v[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {                        // (a part past the last: the last one, weight 0)
+        const long p = min(p0 + k, it.parts - 1) * step;
+        x[k] = ml[p * 32];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k][j] = po[p * (D / 8 * 64) + j * 64];
+      }
+      float mx = m;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, x[k].x);
+      const float use = mx == -INFINITY ? 0.f : mx, old = __builtin_amdgcn_exp2f(m - use);
+      m = mx;
+      l *= old;
+      o *= old;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (p0 + k >= it.parts) break;
+        const float c = __builtin_amdgcn_exp2f(x[k].x - use);
+        l += c * x[k].y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[4 * j + i] += c * v[k][j][i];
+      }
+    }
+    const int row = row0 + r32, qi = row / G;
+    if (row < rows)
+      put_row(a.out + (long)(qbeg + qi) * a.out_stride + (long)(kvh * G + row - qi * G) * D + 8 * h + 32 * dt, o, l != 0.f ? 1.f / l : 0.f);
+  }
+}
+
+}  // namespace
+
+// Rows of a block (a workgroup's) at this head size; 0: not supported.
+EIA_API int eia_quant_flash_rows(int D) {
+  return D == 64 ? Shape<64>::ROWS : D == 128 ? Shape<128>::ROWS : D == 256 ? Shape<256>::ROWS : 0;
+}
+
+// items: n of {sequence, first row, first key, key tiles, slot or -1, 3 unused}; merges: n_merge of {sequence, first row, first slot,
+// parts}; ws: slots * Hkv * rows of a block * (D + 2) floats.
+EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
+                            const void* vs, long codes, long scales, const int* tables, int bt_stride, const int* lens, const int* cu,
+                            const int* items, int n, const int* merges, int n_merge, int slots, float* ws, float scale, int Hq, int Hkv,
+                            int D, int bs, int causal, int window, int chunk, hipStream_t st) {
+  if (n < 0 || n_merge < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || n > 65535 || n_merge > 65535 ||
+      (slots > 0 && !ws))
+    return EIA_BAD_SHAPE;
+  if (n == 0) return EIA_OK;
+  const int groups = bs / QUANT_GROUP, block = eia_quant_flash_rows(D);
+  if (!block) return EIA_UNSUPPORTED;
+  const Chunk a{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, bt_stride, Hq, causal, window, chunk,
+                scale * FLASH_LOG2E, reinterpret_cast<f32x4*>(ws), reinterpret_cast<float2*>(ws + (long)slots * Hkv * block * D), groups,
+                (unsigned)(((1ull << 32) + groups - 1) / groups)};
+  const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
+#define QF_GO(D)                                                                                                                 \
+  do {                                                                                                                           \
+    hipLaunchKernelGGL(quant_flash_kernel<D>, dim3(Hkv, n), dim3(Shape<D>::THREADS), 0, st, a, c, (const Item*)items);           \
+    if (n_merge)                                                                                                                 \
+      hipLaunchKernelGGL(quant_flash_merge_kernel<D>, dim3(Hkv, Shape<D>::THREADS / 64, n_merge), dim3(256), 0, st, a, Hkv, (const Merge*)merges); \
+  } while (0)
+  if (D == 64) QF_GO(64); else if (D == 128) QF_GO(128); else QF_GO(256);
+#undef QF_GO
+  EIA_LAUNCH_CHECK();
+}

@@ -1,0 +1,434 @@
+"""The 8-bit key/value cache: write, read back, decode and chunk attention -> csrc/kernels/quant_*.hip.
+
+A row is the D values of one token and kv head.  With amax its largest magnitude, e is the smallest whole number for which
+amax <= 448 * 2^e, held to [-100, 119]; the row is kept as the e4m3 codes of x / 2^e (nearest, ties to even, at most 448) and one
+byte e + 127.  Every value code * 2^e is exact in bf16.  A token and head of which a key or a value is not finite is marked in
+``k_scale`` by byte 255: both rows read back as NaN, and a query that sees the token becomes NaN.
+
+Step layout, block tables, slots and lengths are those of ``ops.attention`` and ``ops.rotary``.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import dataclasses
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from ._dispatch import check, lib, ptr, require, stream, use_hip
+
+F8 = torch.float8_e4m3fn
+GROUP = 16                    # tokens of a value tile
+ROW_BYTES = 1                 # beside a row's D codes
+HEAD_DIMS = (64, 128, 256)
+UNIT = 64                     # keys that the kernels take at a time
+CUS = 256
+
+
+class QuantKVCache:
+    """One layer's pages: ``k`` [pages, Hkv, page, D] and ``v`` [pages, Hkv, page / 16, D, 16] in e4m3, ``k_scale`` and
+    ``v_scale`` [pages, Hkv, page] bytes.  Pages may lie apart (strides of the first dimension, the same for keys and values);
+    inside a page everything is contiguous."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "num_kv_heads", "block_size", "head_dim", "_args")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        require(k.dim() == 4 and v.dim() == 5, "QuantKVCache: k [pages, Hkv, page, D], v [pages, Hkv, page / 16, D, 16]")
+        n, h, bs, d = k.shape
+        require(bs % GROUP == 0 and bs > 0 and d in HEAD_DIMS, f"QuantKVCache: pages of a multiple of 16 tokens, heads of {HEAD_DIMS}")
+        require(v.shape == (n, h, bs // GROUP, d, GROUP) and k_scale.shape == v_scale.shape == (n, h, bs), "QuantKVCache: shapes")
+        require(k.dtype == v.dtype == F8 and k_scale.dtype == v_scale.dtype == torch.uint8, "QuantKVCache: e4m3 codes, bytes as scales")
+        require(k.device == v.device == k_scale.device == v_scale.device, "QuantKVCache: one device")
+        require(n == 0 or all(t[0].is_contiguous() for t in (k, v, k_scale, v_scale)), "QuantKVCache: a page is contiguous")
+        require(n < 2 or (k.stride(0) == v.stride(0) >= h * bs * d and k_scale.stride(0) == v_scale.stride(0) >= h * bs),
+                "QuantKVCache: keys and values step alike from page to page")
+        require(n * bs < 1 << 31, "QuantKVCache: slots are 32-bit")
+        require(all(t.data_ptr() % 16 == 0 and (n < 2 or t.stride(0) % 16 == 0) for t in (k, v, k_scale, v_scale)),
+                "QuantKVCache: pages begin on 16 bytes")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.num_kv_heads, self.block_size, self.head_dim = n, h, bs, d
+        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0), k_scale.stride(0))
+
+    @classmethod
+    def allocate(cls, pages: int, num_kv_heads: int, block_size: int, head_dim: int, device=None) -> "QuantKVCache":
+        half = num_kv_heads * block_size * (head_dim + ROW_BYTES)
+        require(block_size > 0 and block_size % GROUP == 0, "QuantKVCache: pages of a multiple of 16 tokens")
+        return cls.of_halves(*torch.zeros(2, pages, half, dtype=torch.uint8, device=device), num_kv_heads, block_size, head_dim)
+
+    @classmethod
+    def of_halves(cls, keys: torch.Tensor, values: torch.Tensor, num_kv_heads: int, block_size: int, head_dim: int) -> "QuantKVCache":
+        """Over two byte buffers [pages, Hkv * page * (D + 1)]: a page's codes, then its scales, so that a page is one piece."""
+        h, bs, d = num_kv_heads, block_size, head_dim
+        split = h * bs * d
+        require(keys.dim() == values.dim() == 2 and keys.shape == values.shape and keys.shape[1] == h * bs * (d + ROW_BYTES)
+                and keys.dtype == values.dtype == torch.uint8, "QuantKVCache.of_halves: [pages, Hkv * page * (D + 1)] bytes")
+        codes = [t[:, :split].view(F8) for t in (keys, values)]
+        scales = [t[:, split:].unflatten(1, (h, bs)) for t in (keys, values)]
+        return cls(codes[0].unflatten(1, (h, bs, d)), codes[1].unflatten(1, (h, bs // GROUP, d, GROUP)), *scales)
+
+    @staticmethod
+    def bytes_per_page(num_kv_heads: int, block_size: int, head_dim: int) -> int:
+        return 2 * num_kv_heads * block_size * (head_dim + ROW_BYTES)
+
+
+# ------------------------------------------------------------------------------ plain forms (CPU, and types without kernels)
+def _two_to(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp32 for whole e in [-126, 127]."""
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def quantise_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """fp32 rows [..., D] -> (codes, bytes, whether a value is not finite [...]); rows that are not finite: codes 0, byte 127."""
+    bad = ~torch.isfinite(x).all(-1)
+    x = torch.where(bad.unsqueeze(-1), torch.zeros((), dtype=x.dtype, device=x.device), x)
+    mant, ex = torch.frexp(x.abs().amax(-1))
+    e = (ex - 9 + (mant > 0.875)).clamp(-100, 119)
+    e = torch.where(bad, torch.zeros_like(e), e)
+    return (x * _two_to(-e).unsqueeze(-1)).clamp(-448, 448).to(F8), (e + 127).to(torch.uint8), bad
+
+
+def row_values(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """Codes [..., D] and their bytes -> fp32 values."""
+    e = scale.to(torch.int32) - 127
+    x = codes.float() * _two_to(e.clamp(-100, 119)).unsqueeze(-1)
+    return torch.where((scale == 255).unsqueeze(-1), torch.full((), float("nan"), device=x.device), x)
+
+
+def _write_rows(cache: QuantKVCache, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    keep = (slots >= 0) & (slots < cache.pages * cache.block_size)
+    slots, k, v = slots[keep].long(), k[keep], v[keep]
+    p, t = slots // cache.block_size, slots % cache.block_size
+    kc, kb, kbad = quantise_rows(k)
+    vc, vb, vbad = quantise_rows(v)
+    bad = kbad | vbad
+    kc, vc = (torch.where(bad.unsqueeze(-1), torch.zeros((), dtype=torch.uint8, device=c.device), c.view(torch.uint8)) for c in (kc, vc))
+    cache.k.view(torch.uint8)[p, :, t] = kc
+    cache.v.view(torch.uint8)[p, :, t // GROUP, :, t % GROUP] = vc
+    cache.k_scale[p, :, t] = torch.where(bad, torch.full((), 255, dtype=torch.uint8, device=kb.device), kb)
+    cache.v_scale[p, :, t] = torch.where(bad, torch.full((), 127, dtype=torch.uint8, device=kb.device), vb)
+
+
+def _read_rows(cache: QuantKVCache, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 rows of slots (zeros where a slot is outside the cache)."""
+    there = (slots >= 0) & (slots < cache.pages * cache.block_size)
+    at = torch.where(there, slots, torch.zeros_like(slots)).long()
+    p, t = at // cache.block_size, at % cache.block_size
+    ks = cache.k_scale[p, :, t]
+    vs = torch.where(ks == 255, ks, cache.v_scale[p, :, t])
+    k = row_values(cache.k.view(torch.uint8)[p, :, t].view(F8), ks)
+    v = row_values(cache.v.view(torch.uint8)[p, :, t // GROUP, :, t % GROUP].contiguous().view(F8), vs)
+    gone = ~there[:, None, None]
+    return k.masked_fill(gone, 0.0), v.masked_fill(gone, 0.0)
+
+
+def _rope_rows(qkv, positions, rotary, num_heads, num_kv_heads, head_dim, bias, q_norm_w, k_norm_w, eps):
+    """fp32 (q, k, v) rows of a projection, rotated."""
+    x = qkv.float()
+    if bias is not None:
+        x = x + bias.float()
+    x = x.view(x.shape[0], num_heads + 2 * num_kv_heads, head_dim)
+    qk, v = x[:, :num_heads + num_kv_heads], x[:, num_heads + num_kv_heads:]
+    if q_norm_w is not None:
+        w = torch.cat([q_norm_w.float().expand(num_heads, head_dim), k_norm_w.float().expand(num_kv_heads, head_dim)])
+        qk = qk / torch.sqrt((qk * qk).mean(-1, keepdim=True) + eps) * w
+    if rotary is not None:
+        cs = rotary.cos_sin[positions.long()].unsqueeze(1)
+        c, s = cs[..., :head_dim // 2], cs[..., head_dim // 2:]
+        a, b = (qk[..., :head_dim // 2], qk[..., head_dim // 2:]) if rotary.is_neox else (qk[..., 0::2], qk[..., 1::2])
+        a, b = a * c - b * s, b * c + a * s
+        qk = torch.cat([a, b], -1) if rotary.is_neox else torch.stack([a, b], -1).flatten(-2)
+    return qk[:, :num_heads], qk[:, num_heads:], v
+
+
+def _attend_plain(q, cache, table, L, scale, causal, window, chunk):
+    """q [n, Hq, D], the last n tokens of a sequence of L -> fp32 [n, Hq, D]."""
+    n, Hq, D = q.shape
+    if L <= 0:
+        return torch.zeros(n, Hq, D, device=q.device)
+    j = torch.arange(L, device=q.device)
+    k, v = _read_rows(cache, table[j // cache.block_size].long() * cache.block_size + j % cache.block_size)
+    at = torch.arange(L - n, L, device=q.device).unsqueeze(1)
+    seen = (j <= at) if causal else torch.ones(n, L, dtype=torch.bool, device=q.device)
+    if window:
+        seen = seen & (j > at - window)
+    if chunk:
+        seen = seen & (j >= torch.div(at, chunk, rounding_mode="floor") * chunk)
+    g = Hq // cache.num_kv_heads
+    out = torch.empty(n, Hq, D, device=q.device)
+    for h in range(Hq):
+        s = (q[:, h].float() @ k[:, h // g].T * scale).masked_fill(~seen, float("-inf"))
+        p = torch.softmax(s, -1)
+        p = torch.where(seen.any(-1, keepdim=True), p, torch.zeros_like(p))
+        # a value that nobody sees may be anything
+        vh = torch.where(seen.any(0).unsqueeze(1), v[:, h // g], torch.zeros_like(v[:, h // g]))
+        bad = torch.isnan(vh).any(1)
+        o = p @ vh.masked_fill(bad.unsqueeze(1), 0.0)
+        out[:, h] = o.masked_fill((seen & bad).any(-1, keepdim=True), float("nan"))
+    return out
+
+
+# ------------------------------------------------------------------------------ write and read
+_HERE = contextlib.nullcontext()
+
+
+def _launch_on(t: torch.Tensor):
+    """A launch belongs to the device that is current: the tensors' one."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping: torch.Tensor, cache: QuantKVCache, num_heads: int,
+                   num_kv_heads: int, head_dim: int, bias: Optional[torch.Tensor] = None, q_norm_w: Optional[torch.Tensor] = None,
+                   k_norm_w: Optional[torch.Tensor] = None, norm_eps: float = 1e-6) -> torch.Tensor:
+    """qkv [T, (Hq + 2 Hkv) D] -> q [T, Hq, D]; keys and values go into the 8-bit cache (``rope_qkv_cache`` for it).
+
+    ``qkv`` may be a ``gemm.SplitK``, summed here.  Bias, per-head norms and rotation are fp32, rounded once: queries to bf16,
+    keys and values to their codes.  Slots are distinct; tokens whose slot is outside the cache write nothing."""
+    from .gemm import SplitK
+    part = None
+    if isinstance(qkv, SplitK):
+        if qkv.bias is not None:
+            require(bias is None, "rope_qkv_quant: bias given twice")
+        if use_hip(qkv.part, cache.k):
+            part, bias = qkv, qkv.bias if qkv.bias is not None else bias
+        else:
+            qkv = qkv.materialize()
+    T = part.M if part is not None else qkv.shape[0]
+    width = (num_heads + 2 * num_kv_heads) * head_dim
+    require((part.N if part is not None else qkv.shape[1]) == width, "rope_qkv_quant: qkv width")
+    require(cache.num_kv_heads == num_kv_heads and cache.head_dim == head_dim, "rope_qkv_quant: cache layout")
+    require((q_norm_w is None) == (k_norm_w is None), "rope_qkv_quant: norms of queries and keys together")
+    require(slot_mapping.dtype == torch.int32 and slot_mapping.numel() >= T and slot_mapping.stride(-1) == 1, "slot_mapping int32[T]")
+    if rotary is not None:
+        require(positions is not None and positions.dtype == torch.int32 and positions.numel() >= T and positions.stride(-1) == 1,
+                "positions int32[T]")
+        require(rotary.cos_sin.shape[1] == head_dim and rotary.cos_sin.dtype == torch.float32 and rotary.cos_sin.is_contiguous(),
+                "rope_qkv_quant: cos | sin fp32 [positions, D]")
+    if part is None and not (use_hip(qkv, cache.k) and qkv.dtype == torch.bfloat16):
+        q, k, v = _rope_rows(qkv, None if positions is None else positions[:T], rotary, num_heads, num_kv_heads, head_dim, bias,
+                             q_norm_w, k_norm_w, norm_eps)
+        _write_rows(cache, slot_mapping[:T], k, v)
+        return q.to(qkv.dtype)
+    if part is not None:
+        require(part.part.is_contiguous() and part.part.dtype == torch.float32, "rope_qkv_quant: split-K sums")
+    else:
+        require(qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0, "rope_qkv_quant: rows on 16 bytes")
+    for w, n in ((bias, width), (q_norm_w, head_dim), (k_norm_w, head_dim)):
+        require(w is None or (w.dtype == torch.bfloat16 and w.numel() == n and w.is_contiguous() and w.data_ptr() % 16 == 0),
+                "rope_qkv_quant: bf16 weights on 16 bytes")
+    src = part.part if part is not None else qkv
+    require(all(t is None or t.device == src.device for t in (cache.k, slot_mapping, positions, bias, q_norm_w, k_norm_w)),
+            "rope_qkv_quant: one device")
+    q = torch.empty((T, num_heads, head_dim), dtype=torch.bfloat16, device=src.device)
+    with _launch_on(src):
+        check(lib().eia_quant_write(
+            None if part is not None else ptr(qkv), 0 if part is not None else qkv.stride(0), ptr(src) if part is not None else None,
+            part.sk if part is not None else 0, ptr(positions), None if rotary is None else ptr(rotary.cos_sin), ptr(slot_mapping),
+            *cache._args, cache.pages, ptr(q), ptr(bias), ptr(q_norm_w), ptr(k_norm_w), float(norm_eps), T, num_heads, num_kv_heads,
+            head_dim, cache.block_size, 1 if (rotary is None or rotary.is_neox) else 0, stream(src)), "rope_qkv_quant")
+    return q
+
+
+def quant_read(cache: QuantKVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of the cache's slots (int32 [n]) as (k, v) [n, Hkv, D]: exactly the values kept, zeros where a slot is outside."""
+    require(slots.dtype == torch.int32 and slots.dim() == 1 and slots.is_contiguous(), "quant_read: slots int32 [n]")
+    require(slots.device == cache.k.device, "quant_read: one device")
+    if not (use_hip(slots, cache.k) and dtype == torch.bfloat16):
+        return tuple(t.to(dtype) for t in _read_rows(cache, slots))
+    n = slots.numel()
+    k, v = torch.empty((2, n, cache.num_kv_heads, cache.head_dim), dtype=dtype, device=slots.device)
+    with _launch_on(slots):
+        check(lib().eia_quant_read(*cache._args, cache.pages, ptr(slots), n, ptr(k), ptr(v), cache.num_kv_heads, cache.head_dim,
+                                   cache.block_size, stream(slots)), "quant_read")
+    return k, v
+
+
+# ------------------------------------------------------------------------------ attention
+def _check_attention(name, q, cache, block_tables, seq_lens, scale, out):
+    require(q.dim() == 3 and q.shape[2] == cache.head_dim and q.shape[1] % cache.num_kv_heads == 0, f"{name}: q [tokens, Hq, D]")
+    require(block_tables.dtype == torch.int32 and seq_lens.dtype == torch.int32 and block_tables.dim() == 2, f"{name}: int32 metadata")
+    require(scale > 0.0, f"{name}: scale > 0")
+    require(out is None or (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device), f"{name}: out like q")
+
+
+def _check_hip(name, q, cache, out, *meta):
+    require(q.stride(2) == 1 and q.stride(1) == q.shape[2] and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0, f"{name}: q rows on 16 bytes")
+    require(out.stride(2) == 1 and out.stride(1) == out.shape[2] and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0,
+            f"{name}: out rows on 16 bytes")
+    require(all(t.device == q.device for t in (cache.k, *meta)), f"{name}: one device")
+    require(meta[0].stride(1) == 1 and all(t.stride(-1) == 1 for t in meta[1:]), f"{name}: contiguous metadata")
+
+
+def _row_tiles(rows: int, head_dim: int) -> int:
+    """16-row tiles of the few-rows kernel for so many (query, head) rows; 0: it does not take them."""
+    tiles = -(-rows // 16)
+    return tiles if 1 <= tiles <= (1 if head_dim == 256 else 2) else 0
+
+
+ROW_SLOTS = 2 * CUS           # workgroups of the few-rows kernel that run at a time
+ROW_GRID = 4096               # workgroups of a launch whose lengths the host does not know
+
+
+def _launch_rows(q, out, cache, block_tables, seq_lens, cu, seqs, n, scale, causal, window, chunk, tiles, most, per):
+    Hq, D = q.shape[1], q.shape[2]
+    ws = torch.empty(n * cache.num_kv_heads * most * 16 * tiles * (D + 2), dtype=torch.float32, device=q.device) if most > 1 else None
+    check(lib().eia_quant_rows(
+        ptr(q), q.stride(0), ptr(out), out.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), ptr(seq_lens), cu, seqs, n,
+        float(scale), Hq, cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, most, per,
+        ROW_SLOTS, ptr(ws), stream(q)), "quant_rows")
+
+
+def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                 sliding_window: Optional[int] = None, chunk_size: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [B, Hq, D], one token a sequence, the last of ``seq_lens`` [B] -> out [B, Hq, D] (``paged_decode`` for the 8-bit cache).
+
+    Rows of length 0 become zeros.  Nothing is read back: lengths and tables may change under a captured graph, up to the
+    tables' width."""
+    _check_attention("quant_decode", q, cache, block_tables, seq_lens, scale, out)
+    B, Hq, D = q.shape
+    require(block_tables.shape[0] >= B and seq_lens.numel() >= B, "quant_decode: metadata rows < batch")
+    if not (use_hip(q, cache.k) and q.dtype == torch.bfloat16):
+        rows = [_attend_plain(q[b:b + 1], cache, block_tables[b], int(seq_lens[b]), scale, True, sliding_window, chunk_size) for b in range(B)]
+        r = torch.cat(rows).to(q.dtype) if B else q.clone()
+        return r if out is None else out.copy_(r)
+    o = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
+    _check_hip("quant_decode", q, cache, o, block_tables, seq_lens)
+    tiles = _row_tiles(Hq // cache.num_kv_heads, D)
+    require(tiles > 0, "quant_decode: too many query heads a kv head")
+    if B == 0:
+        return o
+    span = min(w for w in (block_tables.shape[1] * cache.block_size, sliding_window, chunk_size) if w)
+    units = -(-span // UNIT) + (1 if sliding_window or chunk_size else 0)
+    most = max(1, min(-(-units // 4), ROW_GRID // (B * cache.num_kv_heads)))
+    with _launch_on(q):
+        _launch_rows(q, o, cache, block_tables, seq_lens, None, None, B, scale, True, sliding_window, chunk_size, tiles, most, 0)
+    return o
+
+
+@dataclasses.dataclass
+class QuantPrefillPlan:
+    """What a step's chunks have to do, laid out once for all of its layers (``quant_prefill_plan``)."""
+    q_lens: List[int]
+    kv_lens: List[int]
+    num_heads: int
+    num_kv_heads: int
+    head_dim: int
+    causal: bool
+    sliding_window: Optional[int]
+    chunk_size: Optional[int]
+    lists: Optional[torch.Tensor]          # int32: blocks of 8, merges of 4, sequences of few rows
+    n_items: int = 0
+    n_merge: int = 0
+    slots: int = 0
+    n_rows: int = 0
+    row_tiles: int = 1
+    row_parts: int = 1
+    row_per: int = 0
+
+
+def _first_key(at: int, window, chunk) -> int:
+    lo = max(0, at - window + 1) if window else 0
+    return max(lo, at // chunk * chunk) if chunk and at > 0 else lo
+
+
+def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads: int, num_kv_heads: int, head_dim: int, device,
+                       causal: bool = True, sliding_window: Optional[int] = None, chunk_size: Optional[int] = None) -> QuantPrefillPlan:
+    """Work lists of ``quant_prefill`` for chunks of ``q_lens`` new tokens that end at ``kv_lens`` cached ones.
+
+    Sequences of few (query, head) rows go to the kernel that streams the cache for one block of them; the others are cut into
+    blocks of rows, the long ones along the keys too where else the launch would wait for them."""
+    q_lens, kv_lens = [int(n) for n in q_lens], [int(n) for n in kv_lens]
+    require(len(q_lens) == len(kv_lens) and all(n >= 0 for n in q_lens + kv_lens), "quant_prefill_plan: lengths")
+    require(num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim in HEAD_DIMS, "quant_prefill_plan: heads")
+    plan = QuantPrefillPlan(q_lens, kv_lens, num_heads, num_kv_heads, head_dim, causal, sliding_window, chunk_size, None)
+    G = num_heads // num_kv_heads
+    few, blocks = [], []
+    R = 128 if head_dim == 256 else 256
+    total_units = most_units = 0
+    for s, (n, L) in enumerate(zip(q_lens, kv_lens)):
+        if n == 0:
+            continue
+        if _row_tiles(n * G, head_dim):
+            few.append(s)
+            plan.row_tiles = max(plan.row_tiles, _row_tiles(n * G, head_dim))
+            units = -(-L // UNIT) - _first_key(max(L - n, 0), sliding_window, chunk_size) // UNIT if L else 0
+            total_units, most_units = total_units + units, max(most_units, units)
+            continue
+        for r in range(0, n * G, R):
+            first, last = L - n + r // G, L - n + (min(r + R, n * G) - 1) // G
+            hi = min(L, last + 1) if causal else L
+            lo = _first_key(first, sliding_window, chunk_size) // UNIT * UNIT
+            blocks.append((max(0, -(-(hi - lo) // UNIT)), s, r, lo))
+    if few:
+        plan.n_rows = len(few)
+        plan.row_per = max(4, -(-total_units * num_kv_heads // ROW_SLOTS))
+        plan.row_parts = max(1, -(-most_units // plan.row_per))
+    blocks.sort(key=lambda b: -b[0])
+    items, merges = [], []
+    if blocks:
+        per = _flash_per([b[0] for b in blocks], num_kv_heads)
+        for tiles, s, r, lo in blocks:
+            parts = max(1, -(-tiles // per))
+            if parts == 1:
+                items.append((tiles, (s, r, lo, tiles, -1, 0, 0, 0)))
+                continue
+            each = -(-tiles // parts)
+            parts = -(-tiles // each)
+            merges += [s, r, plan.slots, parts]
+            for p in range(parts):
+                t = min(each, tiles - p * each)
+                items.append((t, (s, r, lo + p * each * UNIT, t, plan.slots + p, 0, 0, 0)))
+            plan.slots += parts
+        items.sort(key=lambda b: -b[0])
+        plan.n_items, plan.n_merge = len(items), len(merges) // 4
+    flat = [x for _, it in items for x in it] + merges + few
+    plan.lists = torch.tensor(flat, dtype=torch.int32, device=device)
+    return plan
+
+
+def _flash_per(tiles: List[int], num_kv_heads: int) -> int:
+    """Key tiles of a part at most, for blocks of so many tiles."""
+    work = sum(tiles) * num_kv_heads
+    if len(tiles) * num_kv_heads >= 4 * CUS:
+        return max(tiles + [1])
+    return max(4, -(-work // CUS))
+
+
+def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor,
+                  plan: QuantPrefillPlan, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [T, Hq, D], chunks of new tokens at the end of their sequences (rows cu_q[s] .. cu_q[s + 1]), whose keys and values the
+    cache already holds -> out [T, Hq, D] (``paged_prefill`` for the 8-bit cache).  ``plan`` holds the lengths on the host; rows
+    that see no key become zeros."""
+    _check_attention("quant_prefill", q, cache, block_tables, seq_lens, scale, out)
+    T, Hq, D = q.shape
+    n = len(plan.q_lens)
+    require((plan.num_heads, plan.num_kv_heads, plan.head_dim) == (Hq, cache.num_kv_heads, D), "quant_prefill: plan of other heads")
+    require(sum(plan.q_lens) == T and cu_q.numel() >= n + 1 and cu_q.dtype == torch.int32, "quant_prefill: plan of other chunks")
+    require(block_tables.shape[0] >= n and seq_lens.numel() >= n, "quant_prefill: metadata rows < sequences")
+    require(all(L <= block_tables.shape[1] * cache.block_size for L in plan.kv_lens), "quant_prefill: tables shorter than the sequences")
+    if not (use_hip(q, cache.k) and q.dtype == torch.bfloat16):
+        at, rows = 0, []
+        for s, (m, L) in enumerate(zip(plan.q_lens, plan.kv_lens)):
+            rows.append(_attend_plain(q[at:at + m], cache, block_tables[s], L, scale, plan.causal, plan.sliding_window, plan.chunk_size))
+            at += m
+        r = torch.cat(rows).to(q.dtype) if rows else q.clone()
+        return r if out is None else out.copy_(r)
+    o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
+    _check_hip("quant_prefill", q, cache, o, block_tables, seq_lens, cu_q)
+    if plan.n_items + plan.n_rows == 0:
+        return o
+    require(plan.lists is not None and plan.lists.device == q.device, "quant_prefill: plan of another device")
+    base = plan.lists.data_ptr()
+    with _launch_on(q):
+        if plan.n_items:
+            rows = 128 if D == 256 else 256
+            ws = torch.empty(plan.slots * cache.num_kv_heads * rows * (D + 2), dtype=torch.float32, device=q.device) if plan.slots else None
+            check(lib().eia_quant_flash(
+                ptr(q), q.stride(0), ptr(o), o.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), ptr(seq_lens),
+                ptr(cu_q), base, plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq,
+                cache.num_kv_heads, D, cache.block_size, 1 if plan.causal else 0, plan.sliding_window or 0, plan.chunk_size or 0,
+                stream(q)), "quant_prefill")
+        if plan.n_rows:
+            _launch_rows(q, o, cache, block_tables, seq_lens, ptr(cu_q), base + 32 * plan.n_items + 16 * plan.n_merge, plan.n_rows, scale,
+                         plan.causal, plan.sliding_window, plan.chunk_size, plan.row_tiles, plan.row_parts, plan.row_per)
+    return o

@@ -19,6 +19,14 @@ class RotaryCache:
         self.is_neox = is_neox
         self.cos_sin = ref.rope_cos_sin_cache(max_pos, head_dim, theta, scaling).to(device)
 
+    @classmethod
+    def from_table(cls, cos_sin: torch.Tensor, is_neox: bool = True) -> "RotaryCache":
+        """Over a table [positions, head_dim] fp32 (cos | sin halves) that the caller keeps."""
+        require(cos_sin.dim() == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous(), "RotaryCache: fp32 [positions, D]")
+        self = cls.__new__(cls)
+        self.head_dim, self.is_neox, self.cos_sin = cos_sin.shape[1], is_neox, cos_sin
+        return self
+
 
 def rope_qkv_cache(qkv, positions: Optional[torch.Tensor],
                    rotary: Optional[RotaryCache], slot_mapping: torch.Tensor,
