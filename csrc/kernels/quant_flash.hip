@@ -12,6 +12,9 @@
 //
 // The host lays the launch out (which rows, which tiles): blocks that would be the launch's tail are cut along the keys,
 // their parts hand over fp32 sums and a second kernel puts them together.
+#include <algorithm>
+#include <climits>
+
 #include "eia_flash.h"
 #include "eia_quant.h"
 
@@ -38,7 +41,7 @@ struct Chunk {
   float scale_log2;
   f32x4* po;                         // sums of a part as its lanes hold them [slot][kv head][wave][D / 8][64]
   float2* ml;                        // [slot][kv head][wave][32]
-  int groups;
+  int groups, longest;               // 16-key groups of a page; tokens that a row of the tables has pages for
   unsigned magic;
 };
 
@@ -78,7 +81,7 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r32 = lane & 31, h = lane >> 5;
   const Item it = items[blockIdx.y];
   const int kvh = blockIdx.x, Hkv = cache.Hkv, G = a.Hq / Hkv;
-  const int qbeg = a.cu[it.seq], qlen = a.cu[it.seq + 1] - qbeg, L = a.lens[it.seq], ctx = L - qlen;
+  const int qbeg = a.cu[it.seq], qlen = a.cu[it.seq + 1] - qbeg, L = min(a.lens[it.seq], a.longest), ctx = L - qlen;
   const int rows = qlen * G, row0 = it.row + 32 * w;
   const bool window = a.window > 0 || a.chunk > 0;
   const int row = min(row0 + r32, rows - 1), qi = row / G;
@@ -379,7 +382,7 @@ EIA_API int eia_quant_flash_rows(int D) {
 // items: n of {sequence, first row, first key, key tiles, slot or -1, 3 unused}; merges: n_merge of {sequence, first row, first slot,
 // parts}; ws: slots * Hkv * rows of a block * (D + 2) floats.
 EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
-                            const void* vs, long codes, long scales, const int* tables, int bt_stride, const int* lens, const int* cu,
+                            const void* vs, long codes, long scales, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
                             const int* items, int n, const int* merges, int n_merge, int slots, float* ws, float scale, int Hq, int Hkv,
                             int D, int bs, int causal, int window, int chunk, hipStream_t st) {
   if (n < 0 || n_merge < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || n > 65535 || n_merge > 65535 ||
@@ -390,6 +393,7 @@ EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_st
   if (!block) return EIA_UNSUPPORTED;
   const Chunk a{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, bt_stride, Hq, causal, window, chunk,
                 scale * FLASH_LOG2E, reinterpret_cast<f32x4*>(ws), reinterpret_cast<float2*>(ws + (long)slots * Hkv * block * D), groups,
+                (int)std::min<long>((long)width * bs, INT_MAX),
                 (unsigned)(((1ull << 32) + groups - 1) / groups)};
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
 #define QF_GO(D)                                                                                                                 \

@@ -11,10 +11,20 @@
 //
 // A launch streams the cache once; its keys are cut into parts so that every row block, or a few long ones, load the
 // whole chip.  All workgroups find the same cut from the sequences' lengths (plain sums of them: a few hundred numbers).
+#include <algorithm>
+#include <climits>
+
 #include "eia_flash.h"
 #include "eia_quant.h"
 
 namespace {
+
+// Codes are read once, by one workgroup: they pass the caches by (8 kv heads, 32 rows of up to 16384 keys 164 -> 151 us, 64 of 2048
+// 52.4 -> 47.3).
+EIA_DEV uint4 once(const uint8_t* p) {
+  typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+}
 
 constexpr int RU = 64;               // keys a wave takes at a time
 constexpr int RW = 4;                // waves of a workgroup
@@ -26,9 +36,11 @@ struct Rows {
   const int *tables, *lens, *cu, *list;    // cu: first query of a sequence (nullptr: one each); list: the sequences (nullptr: all)
   int bt_stride, n, Hq, causal, window, chunk;
   float scale_log2;
-  float *po;                         // sums [sequence][kv head][part][column][D]
-  float2* ml;                        // maxima (log2), sums of weights [sequence][kv head][part][column]
-  int most, per, slots, groups;      // parts at most; units a part (0: from all lengths and the workgroups that run at a time); 16-key groups of a page
+  f32x4* po;                         // sums [part][kv head][column][D / 4]
+  float2* ml;                        // maxima (log2), sums of weights [part][kv head][column]
+  int2* info;                        // [sequence]: its first part and their number
+  int per, least, shift, groups;     // units a part (0: by all units, 2^shift workgroups run at a time, `least` at least); 16-key groups of a page
+  int total, longest;                // parts that the launch has room for; tokens that a row of the tables has pages for
   unsigned magic;                    // 2^32 / groups, rounded up
 };
 
@@ -44,40 +56,102 @@ EIA_DEV Span rows_span(const Rows& r, int L, int qlen) {
   return {lo, (L + RU - 1) / RU - lo};
 }
 
-// Units a part: what evens the launch out over the workgroups that run at a time, four (one a wave) at least.
-EIA_DEV int rows_per(const Rows& r, int Hkv) {
-  if (r.per > 0) return r.per;
-  int sum = 0;
-  for (int i = threadIdx.x & 63; i < r.n; i += 64) {
-    const int s = r.list ? r.list[i] : i;
-    sum += rows_span(r, r.lens[s], r.cu ? r.cu[s + 1] - r.cu[s] : 1).units;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  return max(RW, (int)(((long)sum * Hkv + r.slots - 1) / r.slots));
+// Units a part for so many in all: one round of the workgroups that run at a time, or two where that leaves parts of more than
+// RLONG (their ends are apart then).  32 heads on 8, us at 2^8, 2^9, 2^10, 2^11 parts: 65 rows of 1000 to 2000 keys 48.2, 43.9, 45.2,
+// 46.7; 64 of 2048 47.5, 47.4, 50.0, 53.1; 32 of 8192 to 16384 192, 152, 144, 142; 8 of 1000 to 2000 15.5, 12.2, 12.0, 12.2.
+constexpr int RLONG = 48;
+EIA_DEV int rows_per(const Rows& r, long units) {
+  const int one = (int)((units + (1 << r.shift) - 1) >> r.shift), two = (one + 1) / 2;
+  return max(r.least, min(one, max(two, RLONG)));
 }
-EIA_DEV int rows_parts(const Rows& r, int units, int per) { return max(1, min((units + per - 1) / per, r.most)); }
+
+struct Part { int seq, L, q0, qlen, first, index, parts; Span span; };    // seq < 0: none
+
+// The launch's part number y.  Every workgroup finds the same cut from the lengths, 64 sequences at a time: units a part so that
+// the launch evens out over the workgroups that run at a time; a sequence has ceil(units / per) parts,
+// one if it has no units, and parts are numbered through.
+EIA_DEV Part rows_part(const Rows& r, int Hkv, int y) {
+  const int lane = threadIdx.x & 63;
+  auto length = [&](int i, int& s, int& L, int& q0, int& qlen) {
+    s = i < r.n ? (r.list ? r.list[i] : i) : 0;
+    L = i < r.n ? min(r.lens[s], r.longest) : 0;
+    q0 = r.cu ? r.cu[s] : s;
+    qlen = r.cu ? r.cu[s + 1] - q0 : 1;
+  };
+  int s, L, q0, qlen, per = r.per;
+  length(lane, s, L, q0, qlen);
+  if (per == 0) {
+    int sum = 0;
+    for (int i = lane; i < r.n; i += 64) {
+      int s1 = s, L1 = L, q1 = q0, n1 = qlen;
+      if (i != lane) length(i, s1, L1, q1, n1);
+      sum += rows_span(r, L1, n1).units;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    per = rows_per(r, (long)sum * Hkv);
+  }
+  const float inv = 1.f / (float)per;
+  Part found{-1, 0, 0, 0, 0, 0, 0, {0, 0}};
+  for (int i0 = 0, before = 0; i0 < r.n; i0 += 64) {
+    if (i0) length(i0 + lane, s, L, q0, qlen);
+    const Span span = rows_span(r, L, qlen);
+    int parts = (int)((float)span.units * inv);             // ceil(units / per): a float's quotient may be one off
+    parts += parts * per < span.units;
+    parts -= (parts - 1) * per >= span.units;
+    parts = i0 + lane < r.n ? max(parts, 1) : 0;
+    int upto = parts;                                       // inclusive sums over the lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      upto += lane >= o ? x : 0;
+    }
+    const int at = y - before;
+    const unsigned long long mine = __ballot(at >= upto - parts && at < upto);
+    if (mine) {
+      const int from = __builtin_ctzll(mine);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, from); };
+      found = Part{of(s), of(L), of(q0), of(qlen), before + of(upto - parts), 0, of(parts), {of(span.lo), of(span.units)}};
+      found.index = y - found.first;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return found;
+}
+
+EIA_DEV void put_rows(const Rows& r, int q0, int kvh, int G, int D, int col, int d, const f32x4& v, float sum) {
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  bf16x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = f2bf(v[i] * inv);
+  *reinterpret_cast<bf16x4*>(r.out + (long)(q0 + col / G) * r.out_stride + (long)(kvh * G + col % G) * D + d) = y;
+}
 
 template <int D, int NC, bool UNI>
-__global__ void __launch_bounds__(64 * RW, D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(64 * RW, D == 256 || NC == 2 ? 2 : D == 128 ? 3 : 4)
 quant_rows_kernel(Rows r, QuantCache cache) {
   constexpr int KC = D / 64;         // 16-byte pieces of a key row a lane holds
   constexpr int DT = D / 16;
+  constexpr bool AHEAD = D <= 128;   // keys are asked for a unit ahead; 256 channels: that costs the second workgroup on a CU
+  __shared__ bool there;
   __shared__ float sm[RW][16 * NC], sl[RW][16 * NC];
   __shared__ __align__(16) float so[RW][D][16 * NC + 1];
-  const int kvh = blockIdx.x, part = blockIdx.z, Hkv = cache.Hkv, G = r.Hq / Hkv;
-  const int s = r.list ? r.list[blockIdx.y] : blockIdx.y;
+  const int kvh = blockIdx.x, Hkv = cache.Hkv, G = r.Hq / Hkv;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int L = r.lens[s], q0 = r.cu ? r.cu[s] : s, qlen = r.cu ? r.cu[s + 1] - q0 : 1, nrow = min(qlen * G, 16 * NC);
-  const int* bt = r.tables + (long)s * r.bt_stride;
-  const Span span = rows_span(r, L, qlen);
-  const int parts = rows_parts(r, span.units, rows_per(r, Hkv));
-  if (part >= parts || nrow <= 0) return;
+  const Part at = rows_part(r, Hkv, blockIdx.y);
+  const int L = at.L, q0 = at.q0, qlen = at.qlen, nrow = min(qlen * G, 16 * NC), parts = at.parts;
+  if (at.seq < 0) return;
+  if (r.info && at.index == 0 && kvh == 0 && threadIdx.x == 0) r.info[at.seq] = make_int2(at.first, parts);
+  if (nrow <= 0) return;
+  const int* bt = r.tables + (long)at.seq * r.bt_stride;
+  const Span span = at.span;
   const int each = (span.units + parts - 1) / parts;
-  const int ub = span.lo + part * each, ue = min(ub + each, span.lo + span.units);
+  const int ub = span.lo + at.index * each, ue = min(ub + each, span.lo + span.units);
 
-  // Q^T: step 2 i + h of the first product takes channels 64 i + 16 g + 8 h .. + 7 in lane group g
-  bf16x8 qf[NC][2 * KC];
+  // Q^T: step 2 i + h of the first product takes channels 64 i + 16 g + 8 h .. + 7 in lane group g.  In LDS: its registers
+  // are worth a third workgroup on a CU.
+  __shared__ bf16x8 qs[NC][2 * KC][64];
   int kmax[NC], klo[NC];
 #pragma unroll
   for (int t = 0; t < NC; ++t) {
@@ -86,7 +160,8 @@ quant_rows_kernel(Rows r, QuantCache cache) {
 #pragma unroll
     for (int i = 0; i < KC; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) qf[t][2 * i + h] = *reinterpret_cast<const bf16x8*>(qp + 64 * i + 8 * h);
+      for (int h = 0; h < 2; ++h)
+        if (((2 * i + h) & (RW - 1)) == w) qs[t][2 * i + h][lane] = *reinterpret_cast<const bf16x8*>(qp + 64 * i + 8 * h);
     const int qa = L - qlen + qi;
     kmax[t] = r.causal ? min(qa, L - 1) : L - 1;
     klo[t] = 0;
@@ -104,44 +179,58 @@ quant_rows_kernel(Rows r, QuantCache cache) {
     for (int dt = 0; dt < DT; ++dt) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int last = (L - 1) / QUANT_GROUP;                   // the last group with a key: tables end there
-  auto page_of = [&](int group) { return bt[r.groups == 1 ? group : (int)__umulhi((unsigned)group, r.magic)]; };
-  auto off_of = [&](int group) { return QUANT_GROUP * (r.groups == 1 ? 0 : group - (int)__umulhi((unsigned)group, r.magic) * r.groups); };
-  struct Unit {
-    uint4 k[4][KC], v[DT], ks, vs;
+  const int last = max(L - 1, 0) / QUANT_GROUP;                   // the last group with a key: tables end there
+  // 64 pages from one on, a lane each: a unit's page is a register's lane and no load in the loop
+  auto index_of = [&](int group) { return r.groups == 1 ? group : (int)__umulhi((unsigned)group, r.magic); };
+  int held = index_of(min(4 * (ub + w), last));
+  int pages = ub + w < ue ? bt[min(held + lane, index_of(last))] : 0;
+  auto hold = [&](int group) {                              // (the same for the wave)
+    const int at = index_of(group);
+    if (at < held + 60) return;                             // (a unit lies in four pages at most)
+    held = at;
+    pages = bt[min(held + lane, index_of(last))];
   };
-  auto load = [&](Unit& x, int u) {
-    const uint8_t *kp, *vp, *kq, *vq;
-    if constexpr (UNI) {                                    // one page holds the unit
-      const int at = __builtin_amdgcn_readfirstlane(4 * u), off = off_of(at);
-      const int page = __builtin_amdgcn_readfirstlane(page_of(at));
-      kp = cache.key(page, kvh, off, D) + (16 * (c >> 2) + (c & 3)) * D + 16 * g;
-      vp = cache.values(page, kvh, off, D) + 16 * g * D + 16 * c;
-      kq = cache.kscale(page, kvh, off) + 16 * (c >> 2);
-      vq = cache.vscale(page, kvh, off) + 16 * g;
+  auto off_of = [&](int group) { return QUANT_GROUP * (group - index_of(group) * r.groups); };
+  // Where a unit's keys and values lie: page and first token in it, one pair for a unit that one page holds (UNI), else a
+  // pair for the lane's keys and one for its values.
+  struct Place { int pk, ok, pv, ov; };
+  auto look = [&](int u) {
+    Place x;
+    hold(__builtin_amdgcn_readfirstlane(min(4 * u, last)));
+    if constexpr (UNI) {
+      const int at = __builtin_amdgcn_readfirstlane(4 * u);
+      x.ok = x.ov = off_of(at);
+      x.pk = x.pv = __builtin_amdgcn_readlane(pages, index_of(at) - held);
     } else {
       const int gk = min(4 * u + (c >> 2), last), gv = min(4 * u + g, last);
-      const int pk = page_of(gk), pv = page_of(gv), ok = off_of(gk), ov = off_of(gv);
-      kp = cache.key(pk, kvh, ok, D) + (c & 3) * D + 16 * g;
-      vp = cache.values(pv, kvh, ov, D) + 16 * c;
-      kq = cache.kscale(pk, kvh, ok);
-      vq = cache.vscale(pv, kvh, ov);
+      x = Place{__shfl(pages, index_of(gk) - held, 64), off_of(gk), __shfl(pages, index_of(gv) - held, 64), off_of(gv)};
     }
+    return x;
+  };
+  uint4 k[4][KC], ks, v[DT], vs;
+  auto load_keys = [&](const Place& x) {
+    const int page = UNI ? __builtin_amdgcn_readfirstlane(x.pk) : x.pk;
+    const uint8_t* p = cache.key(page, kvh, x.ok, D) + ((UNI ? 16 * (c >> 2) : 0) + (c & 3)) * D + 16 * g;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < KC; ++i) x.k[j][i] = *reinterpret_cast<const uint4*>(kp + 4 * j * D + 64 * i);
-    x.ks = *reinterpret_cast<const uint4*>(kq);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) x.v[dt] = *reinterpret_cast<const uint4*>(vp + 256 * dt);
-    x.vs = *reinterpret_cast<const uint4*>(vq);
+      for (int i = 0; i < KC; ++i) k[j][i] = once(p + 4 * j * D + 64 * i);
+    ks = *reinterpret_cast<const uint4*>(cache.kscale(page, kvh, x.ok) + (UNI ? 16 * (c >> 2) : 0));
   };
-  auto compute = [&](Unit& x, int u) {
+  auto load_values = [&](const Place& x) {
+    const int page = UNI ? __builtin_amdgcn_readfirstlane(x.pv) : x.pv;
+    const uint8_t* p = cache.values(page, kvh, x.ov, D) + (UNI ? 16 * g * D : 0) + 16 * c;
+    vs = *reinterpret_cast<const uint4*>(cache.vscale(page, kvh, x.ov) + (UNI ? 16 * g : 0));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) v[dt] = once(p + 256 * dt);
+  };
+  Place next;
+  auto compute = [&](int u, bool more) {
     // scales of this lane's four key rows
     unsigned kb[4], worst = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      kb[j] = ((&x.ks.x)[j] >> (8 * (c & 3))) & 255u;
+      kb[j] = ((&ks.x)[j] >> (8 * (c & 3))) & 255u;
       worst = max(worst, kb[j]);
     }
     if (__any(worst == QUANT_POISON)) {                     // a token that is no number: every code of its key becomes one
@@ -150,18 +239,18 @@ quant_rows_kernel(Rows r, QuantCache cache) {
         if (kb[j] == QUANT_POISON) {
           kb[j] = 127;
 #pragma unroll
-          for (int i = 0; i < KC; ++i) x.k[j][i] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+          for (int i = 0; i < KC; ++i) k[j][i] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
         }
     }
     if (RU * (u + 1) > L) {                                 // keys past the end: whatever lies there, nothing of it is kept
       const int n = min(max(L - RU * u - 16 * g, 0), 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = min(max(n - 4 * j, 0), 4);
-        const unsigned keep = k == 4 ? ~0u : (1u << (8 * k)) - 1;
-        (&x.vs.x)[j] &= keep;
+        const int left = min(max(n - 4 * j, 0), 4);
+        const unsigned keep = left == 4 ? ~0u : (1u << (8 * left)) - 1;
+        (&vs.x)[j] &= keep;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) (&x.v[dt].x)[j] &= keep;
+        for (int dt = 0; dt < DT; ++dt) (&v[dt].x)[j] &= keep;
       }
     }
     f32x4 sc[NC][4];
@@ -172,14 +261,19 @@ quant_rows_kernel(Rows r, QuantCache cache) {
       for (int t = 0; t < NC; ++t) sc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
-        const bf16x8 a = quant_eight(x.k[j][i].x, x.k[j][i].y, ksc), b = quant_eight(x.k[j][i].z, x.k[j][i].w, ksc);
+        const bf16x8 a = quant_eight(k[j][i].x, k[j][i].y, ksc), b = quant_eight(k[j][i].z, k[j][i].w, ksc);
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
-          sc[t][j] = mfma_bf16_k32(a, qf[t][2 * i], sc[t][j]);
-          sc[t][j] = mfma_bf16_k32(b, qf[t][2 * i + 1], sc[t][j]);
+          sc[t][j] = mfma_bf16_k32(a, qs[t][2 * i][lane], sc[t][j]);
+          sc[t][j] = mfma_bf16_k32(b, qs[t][2 * i + 1][lane], sc[t][j]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    // the next unit's keys take these registers; its values those of this unit's, below
+    __builtin_amdgcn_sched_barrier(0);
+    if (AHEAD && more) load_keys(next);
+    __builtin_amdgcn_sched_barrier(0);
     bf16x8 p[NC][2];
     const bool part_seen = masks || RU * (u + 1) > L;
 #pragma unroll
@@ -208,7 +302,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
         for (int i = 0; i < 4; ++i) {
           const float e = __builtin_amdgcn_exp2f(fmaf(sc[t][j][i], r.scale_log2, -use));
           sum += e;
-          p[t][j >> 1][4 * (j & 1) + i] = f2bf(e * quant_scale(((&x.vs.x)[j] >> (8 * i)) & 255u));
+          p[t][j >> 1][4 * (j & 1) + i] = f2bf(e * quant_scale(((&vs.x)[j] >> (8 * i)) & 255u));
         }
       l[t] = fmaf(l[t], old, sum);
       m[t] = now;
@@ -219,18 +313,34 @@ quant_rows_kernel(Rows r, QuantCache cache) {
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const bf16x8 a = quant_eight(x.v[dt].x, x.v[dt].y, 1.f), b = quant_eight(x.v[dt].z, x.v[dt].w, 1.f);
+      const bf16x8 a = quant_eight(v[dt].x, v[dt].y, 1.f), b = quant_eight(v[dt].z, v[dt].w, 1.f);
 #pragma unroll
       for (int t = 0; t < NC; ++t) {
         o[t][dt] = mfma_bf16_k32(a, p[t][0], o[t][dt]);
         o[t][dt] = mfma_bf16_k32(b, p[t][1], o[t][dt]);
       }
+      if (dt & 1) __builtin_amdgcn_sched_barrier(0);
     }
   };
-  Unit x;
-  for (int u = ub + w; u < ue; u += RW) {
-    load(x, u);
-    compute(x, u);
+  int u = ub + w;
+  if (u < ue) {
+    next = look(u);
+    load_keys(next);
+    load_values(next);
+    if (u + RW < ue) next = look(u + RW);
+  }
+  __syncthreads();
+  if (u < ue) {
+    for (;;) {
+      const bool more = u + RW < ue;
+      compute(u, more);
+      if (!more) break;
+      __builtin_amdgcn_sched_barrier(0);
+      if (!AHEAD) load_keys(next);
+      load_values(next);
+      u += RW;
+      if (u + RW < ue) next = look(u + RW);
+    }
   }
 
 #pragma unroll
@@ -245,7 +355,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
       for (int i = 0; i < 4; ++i) so[w][16 * dt + 4 * g + i][16 * t + c] = o[t][dt][i];
   }
   __syncthreads();
-  const long base = (((long)blockIdx.y * Hkv + kvh) * r.most + part) * (16 * NC);
+  const long base = ((long)blockIdx.y * Hkv + kvh) * (16 * NC);
   for (int id = threadIdx.x; id < nrow * (D / 4); id += 64 * RW) {
     const int col = id / (D / 4), d = id % (D / 4) * 4;
     float mx = sm[0][col];
@@ -262,87 +372,107 @@ quant_rows_kernel(Rows r, QuantCache cache) {
       for (int i = 0; i < 4; ++i) v[i] += so[k][d + i][col] * f;
     }
     if (parts > 1) {
-      *reinterpret_cast<f32x4*>(r.po + (base + col) * D + d) = v;
+      r.po[(base + col) * (D / 4) + d / 4] = v;
       if (d == 0) r.ml[base + col] = make_float2(mx, sum);
     } else {
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;
-      bf16x4 y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = f2bf(v[i] * inv);
-      *reinterpret_cast<bf16x4*>(r.out + (long)(q0 + col / G) * r.out_stride + (long)(kvh * G + col % G) * D + d) = y;
+      put_rows(r, q0, kvh, G, D, col, d, v, sum);
     }
   }
 }
 
+// The parts of a sequence's rows put together: one row a workgroup, D / 4 lanes across it, 1024 / D parts side by side, four of a
+// thread's at a time.
 template <int D, int NC>
 __global__ void __launch_bounds__(256)
 quant_rows_merge_kernel(Rows r, int Hkv) {
-  const int kvh = blockIdx.x, G = r.Hq / Hkv;
+  constexpr int LANES = D / 4, PG = 256 / LANES;
+  __shared__ float sm[PG], sl[PG];
+  __shared__ f32x4 so[PG][LANES];
+  const int kvh = blockIdx.x, G = r.Hq / Hkv, col = blockIdx.z, pg = threadIdx.x / LANES, d = threadIdx.x % LANES;
   const int s = r.list ? r.list[blockIdx.y] : blockIdx.y;
-  const int L = r.lens[s], q0 = r.cu ? r.cu[s] : s, qlen = r.cu ? r.cu[s + 1] - q0 : 1, nrow = min(qlen * G, 16 * NC);
-  const int parts = rows_parts(r, rows_span(r, L, qlen).units, rows_per(r, Hkv));
-  if (parts == 1) return;
-  const long base = ((long)blockIdx.y * Hkv + kvh) * r.most * (16 * NC);
-  for (int id = threadIdx.x; id < nrow * (D / 4); id += 256) {
-    const int col = id / (D / 4), d = id % (D / 4) * 4;
-    float m = -INFINITY, l = 0.f;
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < parts; p0 += 4) {
-      float2 x[4];
-      f32x4 y[4];
+  const int2 at = r.info[s];
+  const int q0 = r.cu ? r.cu[s] : s, qlen = r.cu ? r.cu[s + 1] - q0 : 1, parts = min(at.y, r.total - at.x);
+  if (parts <= 1 || col >= qlen * G) return;
+  const long base = ((long)at.x * Hkv + kvh) * (16 * NC) + col, step = (long)Hkv * (16 * NC);
+  float m = -INFINITY, l = 0.f;
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = pg; p0 < parts; p0 += 4 * PG) {
+    float2 x[4];
+    f32x4 y[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {                         // (a part past the last: the last one, weight 0)
-        const long at = base + (long)min(p0 + k, parts - 1) * (16 * NC) + col;
-        x[k] = r.ml[at];
-        y[k] = *reinterpret_cast<const f32x4*>(r.po + at * D + d);
-      }
-      float mx = m;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, x[k].x);
-      const float use = mx == -INFINITY ? 0.f : mx, old = __builtin_amdgcn_exp2f(m - use);
-      m = mx;
-      l *= old;
-      v *= old;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (p0 + k >= parts) break;
-        const float f = __builtin_amdgcn_exp2f(x[k].x - use);
-        l += x[k].y * f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += y[k][i] * f;
-      }
+    for (int k = 0; k < 4; ++k) {                           // (a part past the last: the last one, weight 0)
+      const long p = base + min(p0 + k * PG, parts - 1) * step;
+      x[k] = r.ml[p];
+      y[k] = r.po[p * LANES + d];
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    bf16x4 y;
+    float mx = m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = f2bf(v[i] * inv);
-    *reinterpret_cast<bf16x4*>(r.out + (long)(q0 + col / G) * r.out_stride + (long)(kvh * G + col % G) * D + d) = y;
+    for (int k = 0; k < 4; ++k) mx = fmaxf(mx, x[k].x);
+    const float use = mx == -INFINITY ? 0.f : mx, old = __builtin_amdgcn_exp2f(m - use);
+    m = mx;
+    l *= old;
+    v *= old;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (p0 + k * PG >= parts) break;
+      const float f = __builtin_amdgcn_exp2f(x[k].x - use);
+      l += x[k].y * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += y[k][i] * f;
+    }
   }
+  so[pg][d] = v;
+  if (d == 0) sm[pg] = m, sl[pg] = l;
+  __syncthreads();
+  if (pg) return;
+  m = sm[0];
+#pragma unroll
+  for (int k = 1; k < PG; ++k) m = fmaxf(m, sm[k]);
+  const float use = m == -INFINITY ? 0.f : m;
+  l = 0.f;
+  v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < PG; ++k) {
+    const float f = __builtin_amdgcn_exp2f(sm[k] - use);
+    l += sl[k] * f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += so[k][d][i] * f;
+  }
+  put_rows(r, q0, kvh, G, D, col, 4 * d, v, l);
 }
 
 }  // namespace
 
-// n sequences (list names them, or the first n), each with at most 16 * tiles rows (query, head of a kv head); most: parts a
-// sequence at most, per: units of 64 keys a part (0: the kernel's own cut); ws: n * Hkv * most * 16 * tiles * (D + 2) floats.
+// n sequences (list names them, or the first n; list entries and `sequences` bound them), each with at most 16 * tiles rows (query,
+// head of a kv head); per: units of 64 keys a part (0: all over 2^shift workgroups, `least` at least); parts: that many at most, n alone if no sequence
+// is cut; ws (parts > n): parts * Hkv * 16 * tiles * (D + 2) floats, then 2 ints for every sequence.
 EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
-                           const void* vs, long codes, long scales, const int* tables, int bt_stride, const int* lens, const int* cu,
+                           const void* vs, long codes, long scales, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
                            const int* list, int n, float scale, int Hq, int Hkv, int D, int bs, int causal, int window, int chunk,
-                           int tiles, int most, int per, int slots, float* ws, hipStream_t st) {
-  if (n < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || most < 1 || (most > 1 && !ws) || n > 65535 || most > 65535 ||
-      slots < 1 || tiles < 1)
+                           int tiles, int parts, int per, int least, int shift, float* ws, hipStream_t st) {
+  if (n < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || parts < n || width < 0 || (parts > n && !ws) || parts > 65535 ||
+      per < 0 || least < 1 || shift < 0 || shift > 24 || tiles < 1)
     return EIA_BAD_SHAPE;
   if (n == 0) return EIA_OK;
   const int groups = bs / QUANT_GROUP;
-  const long sums = (long)n * Hkv * most * 16 * tiles * D;
-  const Rows r{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, list, bt_stride, n, Hq, causal, window, chunk,
-               scale * FLASH_LOG2E, ws, reinterpret_cast<float2*>(ws + sums), most, per, slots, groups,
-               (unsigned)(((1ull << 32) + groups - 1) / groups)};
+  const long rows = (long)parts * Hkv * 16 * tiles;
+  Rows r{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, list, bt_stride, n, Hq, causal, window, chunk,
+         scale * FLASH_LOG2E, nullptr, nullptr, nullptr, per, least, shift, groups, parts,
+         (int)std::min<long>((long)width * bs, INT_MAX), (unsigned)(((1ull << 32) + groups - 1) / groups)};
+  if (parts > n) {
+    r.po = reinterpret_cast<f32x4*>(ws);
+    r.ml = reinterpret_cast<float2*>(ws + rows * D);
+    r.info = reinterpret_cast<int2*>(ws + rows * (D + 2));
+  } else {
+    r.per = 1 << 30;
+  }
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
-#define RW_GO(D, NC)                                                                                                       \
-  do {                                                                                                                     \
-    if (bs % RU == 0) hipLaunchKernelGGL((quant_rows_kernel<D, NC, true>), dim3(Hkv, n, most), dim3(64 * RW), 0, st, r, c); \
-    else hipLaunchKernelGGL((quant_rows_kernel<D, NC, false>), dim3(Hkv, n, most), dim3(64 * RW), 0, st, r, c);             \
-    if (most > 1) hipLaunchKernelGGL((quant_rows_merge_kernel<D, NC>), dim3(Hkv, n), dim3(256), 0, st, r, Hkv);             \
+#define RW_GO(D, NC)                                                                                                      \
+  do {                                                                                                                    \
+    if (bs % RU == 0) hipLaunchKernelGGL((quant_rows_kernel<D, NC, true>), dim3(Hkv, parts), dim3(64 * RW), 0, st, r, c); \
+    else hipLaunchKernelGGL((quant_rows_kernel<D, NC, false>), dim3(Hkv, parts), dim3(64 * RW), 0, st, r, c);             \
+    if (parts > n)                                                                                                        \
+      hipLaunchKernelGGL((quant_rows_merge_kernel<D, NC>), dim3(Hkv, n, cu ? 16 * NC : Hq / Hkv), dim3(256), 0, st, r, Hkv); \
   } while (0)
   if (tiles > (D == 256 ? 1 : 2)) return EIA_UNSUPPORTED;   // (more do not fit the registers)
   switch (D) {

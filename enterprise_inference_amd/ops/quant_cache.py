@@ -265,17 +265,32 @@ def _row_tiles(rows: int, head_dim: int) -> int:
     return tiles if 1 <= tiles <= (1 if head_dim == 256 else 2) else 0
 
 
-ROW_SLOTS = 2 * CUS           # workgroups of the few-rows kernel that run at a time
-ROW_GRID = 4096               # workgroups of a launch whose lengths the host does not know
+ROW_SHIFT = 9                 # 2^9 workgroups share out a launch of the few-rows kernel: two a CU
+ROW_LEAST = 4                 # units a part at least: one a wave
+ROW_LONG = 48                 # longer parts are halved
 
 
-def _launch_rows(q, out, cache, block_tables, seq_lens, cu, seqs, n, scale, causal, window, chunk, tiles, most, per):
+def _launch_rows(q, out, cache, block_tables, seq_lens, cu, seqs, n, sequences, scale, causal, window, chunk, tiles, parts, per):
     Hq, D = q.shape[1], q.shape[2]
-    ws = torch.empty(n * cache.num_kv_heads * most * 16 * tiles * (D + 2), dtype=torch.float32, device=q.device) if most > 1 else None
+    ws = torch.empty(parts * cache.num_kv_heads * 16 * tiles * (D + 2) + 2 * sequences, dtype=torch.float32,
+                     device=q.device) if parts > n else None
     check(lib().eia_quant_rows(
-        ptr(q), q.stride(0), ptr(out), out.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), ptr(seq_lens), cu, seqs, n,
-        float(scale), Hq, cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, most, per,
-        ROW_SLOTS, ptr(ws), stream(q)), "quant_rows")
+        ptr(q), q.stride(0), ptr(out), out.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(seq_lens), cu, seqs, n,
+        float(scale), Hq, cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per,
+        ROW_LEAST, ROW_SHIFT, ptr(ws), stream(q)), "quant_rows")
+
+
+def _rows_per(units: int) -> int:
+    """Units a part for so many of all sequences and kv heads (rows_per in csrc/kernels/quant_rows.hip)."""
+    one = (units + (1 << ROW_SHIFT) - 1) >> ROW_SHIFT
+    return max(ROW_LEAST, min(one, max((one + 1) // 2, ROW_LONG)))
+
+
+def _row_parts(n: int, units: int, num_kv_heads: int) -> int:
+    """Room for the parts of n sequences of at most ``units`` each, whatever their lengths: below one per ``least`` units, and
+    fewer than n more than the workgroups that the units are shared out over."""
+    rounds = 2 if n * units * num_kv_heads > ROW_LONG << ROW_SHIFT else 1
+    return min(n * max(1, -(-units // ROW_LEAST)), (rounds << ROW_SHIFT) // num_kv_heads + n)
 
 
 def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
@@ -299,9 +314,9 @@ def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tenso
         return o
     span = min(w for w in (block_tables.shape[1] * cache.block_size, sliding_window, chunk_size) if w)
     units = -(-span // UNIT) + (1 if sliding_window or chunk_size else 0)
-    most = max(1, min(-(-units // 4), ROW_GRID // (B * cache.num_kv_heads)))
+    parts = _row_parts(B, units, cache.num_kv_heads)
     with _launch_on(q):
-        _launch_rows(q, o, cache, block_tables, seq_lens, None, None, B, scale, True, sliding_window, chunk_size, tiles, most, 0)
+        _launch_rows(q, o, cache, block_tables, seq_lens, None, None, B, B, scale, True, sliding_window, chunk_size, tiles, parts, 0)
     return o
 
 
@@ -344,15 +359,14 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
     G = num_heads // num_kv_heads
     few, blocks = [], []
     R = 128 if head_dim == 256 else 256
-    total_units = most_units = 0
+    units = []
     for s, (n, L) in enumerate(zip(q_lens, kv_lens)):
         if n == 0:
             continue
         if _row_tiles(n * G, head_dim):
             few.append(s)
             plan.row_tiles = max(plan.row_tiles, _row_tiles(n * G, head_dim))
-            units = -(-L // UNIT) - _first_key(max(L - n, 0), sliding_window, chunk_size) // UNIT if L else 0
-            total_units, most_units = total_units + units, max(most_units, units)
+            units.append(-(-L // UNIT) - _first_key(max(L - n, 0), sliding_window, chunk_size) // UNIT if L else 0)
             continue
         for r in range(0, n * G, R):
             first, last = L - n + r // G, L - n + (min(r + R, n * G) - 1) // G
@@ -361,8 +375,8 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
             blocks.append((max(0, -(-(hi - lo) // UNIT)), s, r, lo))
     if few:
         plan.n_rows = len(few)
-        plan.row_per = max(4, -(-total_units * num_kv_heads // ROW_SLOTS))
-        plan.row_parts = max(1, -(-most_units // plan.row_per))
+        plan.row_per = _rows_per(sum(units) * num_kv_heads)
+        plan.row_parts = sum(max(1, -(-u // plan.row_per)) for u in units)
     blocks.sort(key=lambda b: -b[0])
     items, merges = [], []
     if blocks:
@@ -424,11 +438,11 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
             rows = 128 if D == 256 else 256
             ws = torch.empty(plan.slots * cache.num_kv_heads * rows * (D + 2), dtype=torch.float32, device=q.device) if plan.slots else None
             check(lib().eia_quant_flash(
-                ptr(q), q.stride(0), ptr(o), o.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), ptr(seq_lens),
+                ptr(q), q.stride(0), ptr(o), o.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(seq_lens),
                 ptr(cu_q), base, plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq,
                 cache.num_kv_heads, D, cache.block_size, 1 if plan.causal else 0, plan.sliding_window or 0, plan.chunk_size or 0,
                 stream(q)), "quant_prefill")
         if plan.n_rows:
-            _launch_rows(q, o, cache, block_tables, seq_lens, ptr(cu_q), base + 32 * plan.n_items + 16 * plan.n_merge, plan.n_rows, scale,
+            _launch_rows(q, o, cache, block_tables, seq_lens, ptr(cu_q), base + 32 * plan.n_items + 16 * plan.n_merge, plan.n_rows, n, scale,
                          plan.causal, plan.sliding_window, plan.chunk_size, plan.row_tiles, plan.row_parts, plan.row_per)
     return o

@@ -141,13 +141,13 @@ def test_work_lists(heads, hk, d, q_lens, lens, causal, window):
     merges = [flat[at + 4 * i:at + 4 * i + 4] for i in range(plan.n_merge)]
     rows = flat[at + 4 * plan.n_merge:]
     assert len(rows) == plan.n_rows
+    span = lambda s: -(-lens[s] // 64) - (max(0, lens[s] - q_lens[s] - window + 1) // 64 if window else 0)
+    assert plan.row_parts == sum(max(1, -(-span(s) // plan.row_per)) for s in rows) if rows else plan.row_parts == 1
     used = sorted(it[4] for it in items if it[4] >= 0)
     assert used == list(range(plan.slots)) == sorted(m[2] + p for m in merges for p in range(m[3]))
     for s, (n, L) in enumerate(zip(q_lens, lens)):
         assert (s in rows) == (0 < n and -(-n * G // 16) <= (1 if d == 256 else 2))
         if s in rows:
-            units = -(-L // 64)
-            assert plan.row_per * plan.row_parts >= units or window
             continue
         for r in range(0, n * G, R):
             mine = sorted([it for it in items if it[:2] == [s, r]], key=lambda it: it[2])
@@ -160,6 +160,17 @@ def test_work_lists(heads, hk, d, q_lens, lens, causal, window):
             assert (len(mine) > 1) == any(m[:2] == [s, r] and m[3] == len(mine) for m in merges)
     assert sum(1 for it in items) == sum(max(1, sum(m[3] for m in merges if m[:2] == [s, r])) for s, n in enumerate(q_lens) if s not in rows
                                          for r in range(0, n * G, R))
+
+
+def test_room_for_parts():
+    """Decode launches are sized by the tables' width; whatever lengths the kernel finds, its parts have room."""
+    import random
+    r = random.Random(0)
+    for _ in range(20000):
+        n, hk, w = r.choice([1, 2, 3, 8, 65, 200]), r.choice([1, 2, 3, 4, 8, 12, 40, 600]), r.choice([1, 3, 4, 5, 16, 100, 512, 3001])
+        units = [r.choice([0, 1, w, r.randint(0, w)]) for _ in range(n)]
+        per = Q._rows_per(sum(units) * hk)
+        assert sum(max(1, -(-u // per)) for u in units) <= Q._row_parts(n, w, hk)
 
 
 def test_pages_of_two_buffers():
