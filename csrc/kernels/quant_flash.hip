@@ -133,52 +133,56 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
       }
     }
   };
-  auto stash = [&](int buf, int tile) {
-    bf16_t* kl = lds + buf * BUF;
-    bf16_t* vl = kl + FK * KS;
+  // Before the conversion: codes of keys that are no number, values past the end (whatever lies there, nothing of it is kept).
+  auto ready = [&](int tile) {
     const int kb = it.lo + FK * tile;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int id = piece(i);
-      if (keys_here) {
-        uint4 x = kst[i];
-        const bool poison = ksc[i] == QUANT_POISON;        // a token that is no number
-        if (poison) x = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-        const float sc = quant_scale(poison ? 127 : ksc[i]);
-        bf16_t* p = kl + id / (D / 16) * KS + 16 * (id % (D / 16));
-        *reinterpret_cast<bf16x8*>(p) = quant_eight(x.x, x.y, sc);
-        *reinterpret_cast<bf16x8*>(p + 8) = quant_eight(x.z, x.w, sc);
+      if (keys_here && ksc[i] == QUANT_POISON) {
+        ksc[i] = 127;
+        kst[i] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
       }
-      if (values_here) {
-        uint4 x = vst[i];
-        unsigned sb[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sb[j] = __builtin_amdgcn_readfirstlane((&vsc[i].x)[j]);
-        const int group = __builtin_amdgcn_readfirstlane(id / D);
-        if (kb + QUANT_GROUP * (group + 1) > L) {          // keys past the end: whatever lies there, nothing of it is kept
-          const int n = max(L - kb - QUANT_GROUP * group, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int k = min(max(n - 4 * j, 0), 4);
-            const unsigned keep = k == 4 ? ~0u : (1u << (8 * k)) - 1;
-            (&x.x)[j] &= keep;
-            sb[j] &= keep;
-          }
-        }
-        bf16_t* p = vl + id % D * VS + QUANT_GROUP * group;
-        unsigned y[8];
+      if (values_here && kb + FK > L) {
+        const int n = max(L - kb - QUANT_GROUP * (piece(i) / D), 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned word = (&x.x)[j];
-          float s[4];
-#pragma unroll
-          for (int b = 0; b < 4; ++b) s[b] = quant_scale((sb[j] >> (8 * b)) & 255u);
-          y[2 * j] = (quant_pair<false>(word, s[0]) & 0xffffu) | (quant_pair<false>(word, s[1]) & 0xffff0000u);
-          y[2 * j + 1] = (quant_pair<true>(word, s[2]) & 0xffffu) | (quant_pair<true>(word, s[3]) & 0xffff0000u);
+          const int left = min(max(n - 4 * j, 0), 4);
+          const unsigned keep = left == 4 ? ~0u : (1u << (8 * left)) - 1;
+          (&vst[i].x)[j] &= keep;
+          (&vsc[i].x)[j] &= keep;
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(p + 8) = make_uint4(y[4], y[5], y[6], y[7]);
       }
+    }
+  };
+  // Half h of a thread's pieces, converted, into LDS.
+  auto stash = [&](int buf, int i, int h) {
+    bf16_t* kl = lds + buf * BUF;
+    bf16_t* vl = kl + FK * KS;
+    const int id = piece(i);
+    if (keys_here) {
+      bf16_t* p = kl + id / (D / 16) * KS + 16 * (id % (D / 16)) + 8 * h;
+      *reinterpret_cast<bf16x8*>(p) = quant_eight((&kst[i].x)[2 * h], (&kst[i].x)[2 * h + 1], quant_scale(ksc[i]));
+    }
+    if (values_here) {
+      bf16_t* p = vl + id % D * VS + QUANT_GROUP * (id / D) + 8 * h;
+      unsigned y[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned word = (&vst[i].x)[2 * h + j], sb = __builtin_amdgcn_readfirstlane((&vsc[i].x)[2 * h + j]);
+        float s[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) s[b] = quant_scale((sb >> (8 * b)) & 255u);
+        y[2 * j] = (quant_pair<false>(word, s[0]) & 0xffffu) | (quant_pair<false>(word, s[1]) & 0xffff0000u);
+        y[2 * j + 1] = (quant_pair<true>(word, s[2]) & 0xffffu) | (quant_pair<true>(word, s[3]) & 0xffff0000u);
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  };
+  auto stash_all = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      stash(buf, i, 0);
+      stash(buf, i, 1);
     }
   };
 
@@ -190,7 +194,14 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
   float m = -INFINITY, l = 0.f;
   const int krow = swap_bits(r32);
 
-  auto compute = [&](int buf, int kb) {
+  auto ahead = [&](int t) {                                // behind the conversion of tile t + 1: tile t + 2 takes its registers
+    if (t + 2 < it.tiles) {
+      fetch();
+      if (t + 3 < it.tiles) look(t + 3);
+    }
+  };
+  auto compute = [&](int t, int kb) {
+    const int buf = t & 1;
     const bf16_t* kf0 = lds + buf * BUF + krow * KS + 8 * h;
     const bf16_t* vf0 = lds + buf * BUF + FK * KS + r32 * VS + 8 * h;
     f32x16_t sc[2];
@@ -206,14 +217,16 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     for (int b = 0; b < D / 32; ++b) {
       if (b + 1 < D / 32) keys(b + 1);
       __builtin_amdgcn_sched_barrier(0);
+      if (b < 2 * NP) stash(buf ^ 1, b >> 1, b & 1);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int t = 2 * b + (x >> 1);
-        sc[x & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b & 1][x], qf[t], t == 0 ? f32x16_t{} : sc[x & 1], 0, 0, 0);
+        const int step = 2 * b + (x >> 1);
+        sc[x & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b & 1][x], qf[step], step == 0 ? f32x16_t{} : sc[x & 1], 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
+    ahead(t);
     // element i of half sh is key kb + 32 sh + 16 (i / 8) + 8 h + i % 8
     const bool whole = !window && kb + FK <= L && (!a.causal || kb + FK - 1 <= ctx + wq0);
     mfma_settle(sc[0], sc[1]);
@@ -281,22 +294,26 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     __builtin_amdgcn_s_setprio(0);
   };
 
+  // Tile t is multiplied while tile t + 1 is converted, beside the first product, and tile t + 2 is on its way.
   if (it.tiles > 0) {
     look(0);
     fetch();
-    if (it.tiles > 1) look(1);
-    stash(0, 0);
+    look(min(1, it.tiles - 1));
+    ready(0);
+    stash_all(0);
+    if (it.tiles > 1) fetch();
+    if (it.tiles > 2) look(2);
   }
   __syncthreads();
   for (int t = 0; t < it.tiles; ++t) {
     const int kb = it.lo + FK * t;
-    const bool more = t + 1 < it.tiles;
-    if (more) {
-      fetch();
-      if (t + 2 < it.tiles) look(t + 2);
+    ready(t + 1);                                          // (behind the last tile: the same registers into the buffer that nobody reads)
+    if (kb < w_hi && kb + FK > w_lo) {                     // (the same for the wave)
+      compute(t, kb);
+    } else {
+      stash_all((t + 1) & 1);
+      ahead(t);
     }
-    if (kb < w_hi && kb + FK > w_lo) compute(t & 1, kb);   // (the same for the wave)
-    if (more) stash((t + 1) & 1, t + 1);
     __syncthreads();
   }
 
