@@ -261,10 +261,13 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     auto weights = [&](int ks) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(sc[ks >> 1][8 * (ks & 1) + j], a.scale_log2, -use));
-        p[ks][j] = f2bf(e);
-        sum[ks] += e;
+      for (int j = 0; j < 8; j += 2) {
+        const f32x16_t& v = sc[ks >> 1];
+        const int e = 8 * (ks & 1) + j;
+        const bf16x2 y = flash_pack(__builtin_amdgcn_exp2f(fmaf(v[e], a.scale_log2, -use)), __builtin_amdgcn_exp2f(fmaf(v[e + 1], a.scale_log2, -use)));
+        p[ks][j] = y[0];
+        p[ks][j + 1] = y[1];
+        sum[ks] = __builtin_amdgcn_fdot2_f32_bf16(y, bf16x2{(bf16_t)1.f, (bf16_t)1.f}, sum[ks], false);
       }
     };
     constexpr int VB = D / 32 < 4 ? D / 32 : 4;            // fragments of values read ahead

@@ -341,6 +341,9 @@ class QuantPrefillPlan:
     row_per: int = 0
 
 
+FLASH_ROWS = {64: 256, 128: 256, 256: 128}      # (query, head) rows of a workgroup of csrc/kernels/quant_flash.hip
+
+
 def _first_key(at: int, window, chunk) -> int:
     lo = max(0, at - window + 1) if window else 0
     return max(lo, at // chunk * chunk) if chunk and at > 0 else lo
@@ -358,7 +361,7 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
     plan = QuantPrefillPlan(q_lens, kv_lens, num_heads, num_kv_heads, head_dim, causal, sliding_window, chunk_size, None)
     G = num_heads // num_kv_heads
     few, blocks = [], []
-    R = 128 if head_dim == 256 else 256
+    R = FLASH_ROWS[head_dim]
     units = []
     for s, (n, L) in enumerate(zip(q_lens, kv_lens)):
         if n == 0:
@@ -435,8 +438,7 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
     base = plan.lists.data_ptr()
     with _launch_on(q):
         if plan.n_items:
-            rows = 128 if D == 256 else 256
-            ws = torch.empty(plan.slots * cache.num_kv_heads * rows * (D + 2), dtype=torch.float32, device=q.device) if plan.slots else None
+            ws = torch.empty(plan.slots * cache.num_kv_heads * FLASH_ROWS[D] * (D + 2), dtype=torch.float32, device=q.device) if plan.slots else None
             check(lib().eia_quant_flash(
                 ptr(q), q.stride(0), ptr(o), o.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(seq_lens),
                 ptr(cu_q), base, plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq,
