@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import dataclasses
+import heapq
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -383,7 +384,7 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
     blocks.sort(key=lambda b: -b[0])
     items, merges = [], []
     if blocks:
-        per = _flash_per([b[0] for b in blocks], num_kv_heads)
+        per = _flash_per([b[0] for b in blocks], num_kv_heads, head_dim)
         for tiles, s, r, lo in blocks:
             parts = max(1, -(-tiles // per))
             if parts == 1:
@@ -403,12 +404,47 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
     return plan
 
 
-def _flash_per(tiles: List[int], num_kv_heads: int) -> int:
-    """Key tiles of a part at most, for blocks of so many tiles."""
-    work = sum(tiles) * num_kv_heads
-    if len(tiles) * num_kv_heads >= 4 * CUS:
-        return max(tiles + [1])
-    return max(4, -(-work // CUS))
+# MI355X, us: a tile of 64 keys of a workgroup with the chip full, what a workgroup takes besides, a part's sums written and read.
+# (Tiles of 32 workgroups alone take 1.45, 1.8 and 3.1: clocks fall under load.)
+FLASH_TILE = {64: 1.5, 128: 2.1, 256: 3.2}
+FLASH_FIXED = 4.0
+FLASH_PART = {64: 0.02, 128: 0.033, 256: 0.033}
+FLASH_MERGE = 3.0
+
+
+def _makespan(sizes: List[int], slots: int, tile: float) -> float:
+    """Time of a launch whose workgroups of so many tiles (longest first) go to the next slot that is free."""
+    if len(sizes) <= slots:
+        return sizes[0] * tile + FLASH_FIXED
+    ends = [n * tile + FLASH_FIXED for n in sizes[:slots]]
+    heapq.heapify(ends)
+    for n in sizes[slots:]:
+        heapq.heapreplace(ends, ends[0] + n * tile + FLASH_FIXED)
+    return max(ends)
+
+
+def _flash_per(tiles: List[int], num_kv_heads: int, head_dim: int) -> int:
+    """Key tiles of a part at most, for blocks of so many tiles (longest first): what makes the launch shortest, a second kernel
+    and the parts' sums counted.  The kv heads are alike, so one is laid out on its share of the CUs."""
+    slots, tile = max(1, CUS // num_kv_heads), FLASH_TILE[head_dim]
+    longest, work = max(tiles[0], 1), sum(tiles)
+    best, took = longest, _makespan(tiles, slots, tile)
+    if len(tiles) >= 4 * slots:                   # many rounds: they even themselves out
+        return best
+    for rounds in (1, 2, 3, 4, 6):
+        per = max(2, -(-work // (slots * rounds)))
+        if per >= longest:
+            continue
+        sizes, parts = [], 0
+        for n in tiles:
+            k = max(1, -(-n // per))
+            parts += k if k > 1 else 0
+            sizes += [-(-n // k)] * k
+        sizes.sort(reverse=True)
+        t = _makespan(sizes, slots, tile) + FLASH_MERGE + parts * num_kv_heads * FLASH_PART[head_dim]
+        if t < took:
+            best, took = per, t
+    return best
 
 
 def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor,
