@@ -265,7 +265,9 @@ class CacheConfig:
     cpu_kvcache_space_gb: float = 4.0        # VLLM_CPU_KVCACHE_SPACE analogue
     swap_space_gb: float = 4.0               # --swap-space: pinned host KV for preemption
     enable_prefix_caching: bool = True
-    cache_dtype: Optional[torch.dtype] = None   # None -> model dtype
+    # None -> model dtype; torch.float8_e4m3fn -> e4m3 codes with one power-of-two scale per token
+    # and kv head (ops/quant_cache.py)
+    cache_dtype: Optional[torch.dtype] = None
     # per-sequence state slots of recurrent layers (0: the model has none); set by EngineConfig
     # to max_num_seqs for models that need them, which also turns prefix caching off
     num_state_slots: int = 0
@@ -355,6 +357,12 @@ class EngineConfig:
             self.enforce_eager = True        # host-staged gloo collectives cannot be captured
         if self.cache.cache_dtype is None:
             self.cache.cache_dtype = self.dtype
+        if self.cache.cache_dtype == torch.float8_e4m3fn:
+            if self._model_attr("allocate_cache"):
+                raise ValueError("the 8-bit KV cache is for models with the common key/value cache, not "
+                                 "for those that lay out their own")
+            if self.model.head_dim not in (64, 128, 256):
+                raise ValueError(f"the 8-bit KV cache takes heads of 64, 128 or 256, not {self.model.head_dim}")
         if self._model_attr("needs_state_slots") and not self.cache.num_state_slots:
             self.cache.num_state_slots = self.scheduler.max_num_seqs
         if self.scheduler.max_model_len > self.model.max_position_embeddings and \

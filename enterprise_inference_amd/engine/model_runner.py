@@ -25,6 +25,7 @@ from ..config import EngineConfig
 from ..models.loader import build_model
 from ..ops import attention as attn_ops
 from ..ops import sampling as sampling_ops
+from ..ops.quant_cache import QuantKVCache
 from ..parallel import state as pstate
 from .block_manager import BlockManager
 from .scheduler import ScheduledSeq, SchedulerOutput
@@ -191,6 +192,7 @@ class ModelRunner:
         # models that lay out their own caches (latent rows, recurrent state slots) allocate
         # them through allocate_cache(); the block tables, slots and batching stay the same
         self.custom_cache = hasattr(self.model, "allocate_cache")
+        self.quant_cache = not self.custom_cache and cfg.cache.cache_dtype == torch.float8_e4m3fn
         self.num_state_slots = cfg.cache.num_state_slots if getattr(
             self.model, "needs_state_slots", False) else 0
         self.kv_buf = None
@@ -329,6 +331,9 @@ class ModelRunner:
     def kv_block_bytes(self) -> int:
         if self.custom_cache:
             return int(self.model.cache_block_bytes(self.block_size, self.cfg.cache.cache_dtype))
+        if self.quant_cache:
+            return self.num_local_layers * QuantKVCache.bytes_per_page(
+                self.num_kv_heads, self.block_size, self.head_dim)
         e = torch.tensor([], dtype=self.cfg.cache.cache_dtype).element_size()
         return self.num_local_layers * 2 * self.num_kv_heads * self.block_size * self.head_dim * e
 
@@ -364,6 +369,8 @@ class ModelRunner:
         pos = torch.arange(n, dtype=torch.int32, device=self.device) % self.cfg.scheduler.max_model_len
         slots = torch.full((n,), -1, dtype=torch.int32, device=self.device)
         # scratch 1-block caches suffice (slots < 0: no writes)
+        kv = QuantKVCache.allocate(1, self.num_kv_heads, self.block_size, self.head_dim,
+                                   self.device) if self.quant_cache else None
         k = torch.zeros(1, self.num_kv_heads, self.block_size, self.head_dim, dtype=self.cfg.dtype,
                         device=self.device)
         v = torch.zeros(1, self.num_kv_heads, self.head_dim, self.block_size, dtype=self.cfg.dtype,
@@ -400,7 +407,7 @@ class ModelRunner:
             if self.pp > 1 and not pstate.is_first_stage():
                 z = torch.zeros(n, self.hidden_size, dtype=self.cfg.dtype, device=self.device)
                 inter = (z, z.clone())
-            h = self._forward(ids, md, [(k, v)] * self.num_layers, inter)
+            h = self._forward(ids, md, [kv or (k, v)] * self.num_layers, inter)
             if self.pp == 1 or pstate.is_last_stage():
                 idx = torch.arange(min(n, self.max_num_seqs), device=self.device)
                 self.model.compute_logits(h[idx])
@@ -416,6 +423,17 @@ class ModelRunner:
                         nb, self.block_size, self.num_state_slots)
             return nb
         Hkv, bs, D = self.num_kv_heads, self.block_size, self.head_dim
+        if self.quant_cache:
+            # a block's codes and scales are one piece, so swaps and copies move bytes of blocks
+            half = QuantKVCache.bytes_per_page(Hkv, bs, D) // 2
+            buf = torch.zeros(self.num_local_layers, 2, nb * half, dtype=torch.uint8, device=self.device)
+            self.kv_buf = buf
+            self.kv_caches = [QuantKVCache.of_halves(*buf[l - self.layer_lo].view(2, nb, half), Hkv, bs, D)
+                              if self.layer_lo <= l < self.layer_hi else None
+                              for l in range(self.num_layers)]
+            logger.info("KV cache: %d blocks x %d tokens, 8 bits a value (%.1f GiB)", nb, bs,
+                        buf.numel() / 2**30)
+            return nb
         per_layer = nb * Hkv * bs * D
         # zero-filled: never-written slots must stay finite (masked P=0 times V)
         # only this pipeline stage's layers get cache memory (others: None)
@@ -432,8 +450,7 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ swap (K14)
     def kv_bytes_per_block(self) -> int:
-        return 2 * self.num_local_layers * self.num_kv_heads * self.block_size * \
-            self.head_dim * self.kv_buf.element_size()
+        return self.kv_buf.numel() // self.num_blocks * self.kv_buf.element_size()
 
     def allocate_swap(self, num_cpu_blocks: int) -> int:
         """Pinned host swap space, block-major [cpu_blocks, layers, 2, block elems]: every
@@ -672,6 +689,7 @@ class ModelRunner:
         if npf:
             md.prefill_qblock = self._query_block()
             md.prefill_q_lens = np.diff(self.e_buf.numpy()[o["cu"]:o["cu"] + npf + 1]).tolist()
+            md.prefill_kv_lens = self.e_buf.numpy()[o["plen"]:o["plen"] + npf].tolist()
         if "sslot" in o:
             ns = nd + npf
             md.num_seqs = ns

@@ -20,6 +20,7 @@ import torch.nn.functional as F
 from ..config import ModelConfig
 from ..ops import activation, gemm  # noqa: F401
 from ..ops.attention import AttentionMetadata, attention, decode_rope_attention
+from ..ops.quant_cache import QuantKVCache, quant_attention, rope_qkv_quant
 from ..ops.rotary import RotaryCache, rope_qkv_cache
 from ..parallel import state
 from ..ops.gemm import SplitK
@@ -62,6 +63,12 @@ class LlamaAttention(nn.Module):
         qkv = gemm.linear(h, self.qkv_proj.weight, defer_reduce=True)   # split-K summed in K4
         qn = None if self.q_norm is None else self.q_norm.weight
         kn = None if self.k_norm is None else self.k_norm.weight
+        if isinstance(kv, QuantKVCache):
+            q = rope_qkv_quant(qkv, md.positions, self.rotary, md.slot_mapping, kv, self.num_heads,
+                               self.num_kv_heads, self.head_dim, bias=self.qkv_proj.bias,
+                               q_norm_w=qn, k_norm_w=kn, norm_eps=self.cfg.rms_norm_eps)
+            o = quant_attention(q, kv, md, self.scale, self.sliding_window, self.chunk_size)
+            return self.o_proj(o.view(-1, self.num_heads * self.head_dim)[:T], defer_reduce=True)
         # pure decode: K4 (reduce/bias/qk-norm/RoPE/KV write) runs inside the attention kernel
         o = decode_rope_attention(qkv, md, kv[0], kv[1], self.rotary, self.num_heads,
                                   self.num_kv_heads, self.head_dim, self.scale,

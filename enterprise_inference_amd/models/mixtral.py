@@ -442,18 +442,21 @@ class Llama4Attention(LlamaAttention):
 
     def forward(self, h, md, kv):
         from ..ops.attention import attention
+        from ..ops.quant_cache import QuantKVCache, quant_attention, rope_qkv_quant
         from ..ops.rotary import rope_qkv_cache
         from ..ops import gemm
 
         T = h.shape[0]
         # split-K QKV slabs are summed inside the RoPE / KV-write kernel (no reduce launch)
         qkv = gemm.linear(h, self.qkv_proj.weight, defer_reduce=True)
-        q = rope_qkv_cache(qkv, md.positions, self.rotary, md.slot_mapping, kv[0], kv[1],
-                           self.num_heads, self.num_kv_heads, self.head_dim,
-                           bias=self.qkv_proj.bias,
-                           q_norm_w=self.ones if self.qk_l2 else None,
-                           k_norm_w=self.ones if self.qk_l2 else None,
-                           norm_eps=self.cfg.rms_norm_eps)
+        quant = isinstance(kv, QuantKVCache)
+        write, where = (rope_qkv_quant, (kv,)) if quant else (rope_qkv_cache, (kv[0], kv[1]))
+        q = write(qkv, md.positions, self.rotary, md.slot_mapping, *where,
+                  self.num_heads, self.num_kv_heads, self.head_dim,
+                  bias=self.qkv_proj.bias,
+                  q_norm_w=self.ones if self.qk_l2 else None,
+                  k_norm_w=self.ones if self.qk_l2 else None,
+                  norm_eps=self.cfg.rms_norm_eps)
         if self.temp_tuning:
             # the per-position temperature is the same for every NoPE layer of the step:
             # computed once per step (cached on the step's metadata), applied in fp32
@@ -466,7 +469,10 @@ class Llama4Attention(LlamaAttention):
                 cached = (key, sc[:, None, None])
                 md._l4_attn_temp = cached
             q = (q * cached[1]).to(q.dtype)
-        o = attention(q, kv[0], kv[1], md, self.scale, None, self.chunk_size)
+        if quant:
+            o = quant_attention(q, kv, md, self.scale, None, self.chunk_size)
+        else:
+            o = attention(q, kv[0], kv[1], md, self.scale, None, self.chunk_size)
         return self.o_proj(o.view(T, self.num_heads * self.head_dim), defer_reduce=True)
 
 

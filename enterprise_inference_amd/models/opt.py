@@ -17,6 +17,7 @@ import torch.nn as nn
 from ..config import ModelConfig
 from ..ops import activation as act_ops
 from ..ops.attention import AttentionMetadata, attention
+from ..ops.quant_cache import QuantKVCache, quant_attention, rope_qkv_quant
 from ..ops.rotary import rope_qkv_cache
 from .layers import (ColumnParallelLinear, LayerNorm, ParallelLMHead, QKVParallelLinear,
                      ReplicatedLinear, RowParallelLinear, VocabParallelEmbedding, _param,
@@ -37,9 +38,14 @@ class OPTAttention(nn.Module):
     def forward(self, h, md: AttentionMetadata, kv):
         T = h.shape[0]
         qkv = self.qkv_proj(h)
-        q = rope_qkv_cache(qkv, md.positions, None, md.slot_mapping, kv[0], kv[1], self.nh,
-                           self.nkv, self.hd)
-        o = attention(q, kv[0], kv[1], md, self.scale)
+        if isinstance(kv, QuantKVCache):
+            q = rope_qkv_quant(qkv, md.positions, None, md.slot_mapping, kv, self.nh, self.nkv,
+                               self.hd)
+            o = quant_attention(q, kv, md, self.scale)
+        else:
+            q = rope_qkv_cache(qkv, md.positions, None, md.slot_mapping, kv[0], kv[1], self.nh,
+                               self.nkv, self.hd)
+            o = attention(q, kv[0], kv[1], md, self.scale)
         return self.out_proj(o.reshape(T, self.nh * self.hd))
 
 

@@ -253,6 +253,7 @@ class AttentionMetadata:
     prefill_n_work: int = 0
     prefill_qblock: int = 0                              # queries per work item (0: not stated)
     prefill_q_lens: Optional[List[int]] = None           # host copy of the chunk lengths
+    prefill_kv_lens: Optional[List[int]] = None          # and of prefill_seq_lens
     causal: bool = True
     # multimodal: batch rows whose token embedding is replaced (image placeholders)
     mm_rows: Optional[torch.Tensor] = None               # [n] int64
@@ -262,7 +263,8 @@ class AttentionMetadata:
     num_seqs: int = 0
     seq_slots: Optional[torch.Tensor] = None             # [num_seqs] int32 (< 0: padding row)
     seq_cu: Optional[torch.Tensor] = None                # [num_seqs + 1] int32
-    # work lists for kernels whose query block differs from prefill_qblock: qblock -> (list, n)
+    # work lists for kernels whose query block differs from prefill_qblock: qblock -> (list, n); plans of
+    # quant_cache.quant_attention
     work_cache: dict = dataclasses.field(default_factory=dict)
 
     def prefill_work_for(self, qblock: int, build):

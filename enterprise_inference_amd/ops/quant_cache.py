@@ -10,14 +10,13 @@ Step layout, block tables, slots and lengths are those of ``ops.attention`` and 
 
 from __future__ import annotations
 
-import contextlib
 import dataclasses
 import heapq
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from ._dispatch import check, lib, ptr, require, stream, use_hip
+from ._dispatch import check, lib, ptr, require, use_hip
 
 F8 = torch.float8_e4m3fn
 GROUP = 16                    # tokens of a value tile
@@ -32,7 +31,7 @@ class QuantKVCache:
     ``v_scale`` [pages, Hkv, page] bytes.  Pages may lie apart (strides of the first dimension, the same for keys and values);
     inside a page everything is contiguous."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "num_kv_heads", "block_size", "head_dim", "_args")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "num_kv_heads", "block_size", "head_dim", "device", "_hip", "_args")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         require(k.dim() == 4 and v.dim() == 5, "QuantKVCache: k [pages, Hkv, page, D], v [pages, Hkv, page / 16, D, 16]")
@@ -49,6 +48,7 @@ class QuantKVCache:
                 "QuantKVCache: pages begin on 16 bytes")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.num_kv_heads, self.block_size, self.head_dim = n, h, bs, d
+        self.device, self._hip = k.device, use_hip(k)
         self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0), k_scale.stride(0))
 
     @classmethod
@@ -170,12 +170,14 @@ def _attend_plain(q, cache, table, L, scale, causal, window, chunk):
 
 
 # ------------------------------------------------------------------------------ write and read
-_HERE = contextlib.nullcontext()
-
-
-def _launch_on(t: torch.Tensor):
-    """A launch belongs to the device that is current: the tensors' one."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(name: str, call, device: torch.device, *args) -> None:
+    """``call`` on the device's current stream.  A launch belongs to the device that is current: the tensors' one."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        check(call(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+    else:
+        with torch.cuda.device(index):
+            check(call(*args, torch._C._cuda_getCurrentRawStream(index)), name)
 
 
 def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping: torch.Tensor, cache: QuantKVCache, num_heads: int,
@@ -185,79 +187,95 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
 
     ``qkv`` may be a ``gemm.SplitK``, summed here.  Bias, per-head norms and rotation are fp32, rounded once: queries to bf16,
     keys and values to their codes.  Slots are distinct; tokens whose slot is outside the cache write nothing."""
-    from .gemm import SplitK
     part = None
-    if isinstance(qkv, SplitK):
+    if not isinstance(qkv, torch.Tensor):
+        from .gemm import SplitK
+        require(isinstance(qkv, SplitK), "rope_qkv_quant: a tensor or split-K sums")
         if qkv.bias is not None:
             require(bias is None, "rope_qkv_quant: bias given twice")
-        if use_hip(qkv.part, cache.k):
+        if cache._hip and qkv.part.is_cuda:
             part, bias = qkv, qkv.bias if qkv.bias is not None else bias
+            require(part.part.is_contiguous() and part.part.dtype == torch.float32, "rope_qkv_quant: split-K sums")
         else:
             qkv = qkv.materialize()
-    T = part.M if part is not None else qkv.shape[0]
+    T, N = (part.M, part.N) if part is not None else qkv.shape
     width = (num_heads + 2 * num_kv_heads) * head_dim
-    require((part.N if part is not None else qkv.shape[1]) == width, "rope_qkv_quant: qkv width")
-    require(cache.num_kv_heads == num_kv_heads and cache.head_dim == head_dim, "rope_qkv_quant: cache layout")
-    require((q_norm_w is None) == (k_norm_w is None), "rope_qkv_quant: norms of queries and keys together")
-    require(slot_mapping.dtype == torch.int32 and slot_mapping.numel() >= T and slot_mapping.stride(-1) == 1, "slot_mapping int32[T]")
+    if not (N == width and cache.num_kv_heads == num_kv_heads and cache.head_dim == head_dim):
+        raise ValueError("rope_qkv_quant: qkv width, cache layout")
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise ValueError("rope_qkv_quant: norms of queries and keys together")
+    if not (slot_mapping.dtype is torch.int32 and slot_mapping.numel() >= T and slot_mapping.stride(-1) == 1):
+        raise ValueError("rope_qkv_quant: slot_mapping int32[T]")
+    table, neox = None, True
     if rotary is not None:
-        require(positions is not None and positions.dtype == torch.int32 and positions.numel() >= T and positions.stride(-1) == 1,
-                "positions int32[T]")
-        require(rotary.cos_sin.shape[1] == head_dim and rotary.cos_sin.dtype == torch.float32 and rotary.cos_sin.is_contiguous(),
-                "rope_qkv_quant: cos | sin fp32 [positions, D]")
-    if part is None and not (use_hip(qkv, cache.k) and qkv.dtype == torch.bfloat16):
+        table, neox = rotary.cos_sin, rotary.is_neox
+        if not (positions is not None and positions.dtype is torch.int32 and positions.numel() >= T and positions.stride(-1) == 1):
+            raise ValueError("rope_qkv_quant: positions int32[T]")
+        if not (table.shape[1] == head_dim and table.dtype is torch.float32 and table.is_contiguous()):
+            raise ValueError("rope_qkv_quant: cos | sin fp32 [positions, D]")
+    src = part.part if part is not None else qkv
+    if part is None and not (cache._hip and qkv.is_cuda and qkv.dtype is torch.bfloat16):
         q, k, v = _rope_rows(qkv, None if positions is None else positions[:T], rotary, num_heads, num_kv_heads, head_dim, bias,
                              q_norm_w, k_norm_w, norm_eps)
         _write_rows(cache, slot_mapping[:T], k, v)
         return q.to(qkv.dtype)
-    if part is not None:
-        require(part.part.is_contiguous() and part.part.dtype == torch.float32, "rope_qkv_quant: split-K sums")
-    else:
-        require(qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0, "rope_qkv_quant: rows on 16 bytes")
+    if part is None and not (qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0):
+        raise ValueError("rope_qkv_quant: rows on 16 bytes")
     for w, n in ((bias, width), (q_norm_w, head_dim), (k_norm_w, head_dim)):
-        require(w is None or (w.dtype == torch.bfloat16 and w.numel() == n and w.is_contiguous() and w.data_ptr() % 16 == 0),
-                "rope_qkv_quant: bf16 weights on 16 bytes")
-    src = part.part if part is not None else qkv
-    require(all(t is None or t.device == src.device for t in (cache.k, slot_mapping, positions, bias, q_norm_w, k_norm_w)),
-            "rope_qkv_quant: one device")
-    q = torch.empty((T, num_heads, head_dim), dtype=torch.bfloat16, device=src.device)
-    with _launch_on(src):
-        check(lib().eia_quant_write(
-            None if part is not None else ptr(qkv), 0 if part is not None else qkv.stride(0), ptr(src) if part is not None else None,
-            part.sk if part is not None else 0, ptr(positions), None if rotary is None else ptr(rotary.cos_sin), ptr(slot_mapping),
-            *cache._args, cache.pages, ptr(q), ptr(bias), ptr(q_norm_w), ptr(k_norm_w), float(norm_eps), T, num_heads, num_kv_heads,
-            head_dim, cache.block_size, 1 if (rotary is None or rotary.is_neox) else 0, stream(src)), "rope_qkv_quant")
+        if w is not None and not (w.dtype is torch.bfloat16 and w.numel() == n and w.is_contiguous() and w.data_ptr() % 16 == 0):
+            raise ValueError("rope_qkv_quant: bf16 weights on 16 bytes")
+    device = src.device
+    if not all(t is None or t.device == device for t in (cache, slot_mapping, positions if table is not None else None, table, bias, q_norm_w,
+                                                         k_norm_w)):
+        raise ValueError("rope_qkv_quant: one device")
+    q = torch.empty((T, num_heads, head_dim), dtype=torch.bfloat16, device=device)
+    _launch("rope_qkv_quant", lib().eia_quant_write, device, None if part is not None else ptr(qkv),
+            0 if part is not None else qkv.stride(0), ptr(src) if part is not None else None, part.sk if part is not None else 0,
+            ptr(positions), ptr(table), ptr(slot_mapping), *cache._args, cache.pages, ptr(q), ptr(bias), ptr(q_norm_w), ptr(k_norm_w),
+            float(norm_eps), T, num_heads, num_kv_heads, head_dim, cache.block_size, 1 if neox else 0)
     return q
 
 
 def quant_read(cache: QuantKVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows of the cache's slots (int32 [n]) as (k, v) [n, Hkv, D]: exactly the values kept, zeros where a slot is outside."""
-    require(slots.dtype == torch.int32 and slots.dim() == 1 and slots.is_contiguous(), "quant_read: slots int32 [n]")
-    require(slots.device == cache.k.device, "quant_read: one device")
-    if not (use_hip(slots, cache.k) and dtype == torch.bfloat16):
+    if not (slots.dtype is torch.int32 and slots.dim() == 1 and slots.is_contiguous() and slots.device == cache.device):
+        raise ValueError("quant_read: slots int32 [n] on the cache's device")
+    if not (cache._hip and dtype is torch.bfloat16):
         return tuple(t.to(dtype) for t in _read_rows(cache, slots))
-    n = slots.numel()
-    k, v = torch.empty((2, n, cache.num_kv_heads, cache.head_dim), dtype=dtype, device=slots.device)
-    with _launch_on(slots):
-        check(lib().eia_quant_read(*cache._args, cache.pages, ptr(slots), n, ptr(k), ptr(v), cache.num_kv_heads, cache.head_dim,
-                                   cache.block_size, stream(slots)), "quant_read")
+    shape = (slots.shape[0], cache.num_kv_heads, cache.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=cache.device)
+    v = torch.empty(shape, dtype=dtype, device=cache.device)
+    _launch("quant_read", lib().eia_quant_read, cache.device, *cache._args, cache.pages, slots.data_ptr(), shape[0], k.data_ptr(),
+            v.data_ptr(), shape[1], shape[2], cache.block_size)
     return k, v
 
 
 # ------------------------------------------------------------------------------ attention
-def _check_attention(name, q, cache, block_tables, seq_lens, scale, out):
-    require(q.dim() == 3 and q.shape[2] == cache.head_dim and q.shape[1] % cache.num_kv_heads == 0, f"{name}: q [tokens, Hq, D]")
-    require(block_tables.dtype == torch.int32 and seq_lens.dtype == torch.int32 and block_tables.dim() == 2, f"{name}: int32 metadata")
-    require(scale > 0.0, f"{name}: scale > 0")
-    require(out is None or (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device), f"{name}: out like q")
-
-
-def _check_hip(name, q, cache, out, *meta):
-    require(q.stride(2) == 1 and q.stride(1) == q.shape[2] and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0, f"{name}: q rows on 16 bytes")
-    require(out.stride(2) == 1 and out.stride(1) == out.shape[2] and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0,
-            f"{name}: out rows on 16 bytes")
-    require(all(t.device == q.device for t in (cache.k, *meta)), f"{name}: one device")
-    require(meta[0].stride(1) == 1 and all(t.stride(-1) == 1 for t in meta[1:]), f"{name}: contiguous metadata")
+def _check_attention(name, q, cache, block_tables, seq_lens, n, scale, out):
+    """(whether the kernels take it, tokens, heads); ``n`` sequences."""
+    T, Hq, D = q.shape
+    if not (D == cache.head_dim and Hq % cache.num_kv_heads == 0):
+        raise ValueError(f"{name}: q [tokens, Hq, D]")
+    if not (block_tables.dtype is torch.int32 and seq_lens.dtype is torch.int32 and block_tables.dim() == 2):
+        raise ValueError(f"{name}: int32 metadata")
+    if not (block_tables.shape[0] >= n and seq_lens.numel() >= n):
+        raise ValueError(f"{name}: metadata rows < sequences")
+    if not scale > 0.0:
+        raise ValueError(f"{name}: scale > 0")
+    if out is not None and not (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device):
+        raise ValueError(f"{name}: out like q")
+    if not (cache._hip and q.is_cuda and q.dtype is torch.bfloat16):
+        return False, T, Hq
+    for t in (q, out):
+        if t is not None:
+            s = t.stride()
+            if not (s[2] == 1 and s[1] == D and s[0] % 8 == 0 and t.data_ptr() % 16 == 0):
+                raise ValueError(f"{name}: rows of q and out on 16 bytes")
+    if not (q.device == cache.device == block_tables.device == seq_lens.device):
+        raise ValueError(f"{name}: one device")
+    if not (block_tables.stride(1) == 1 and seq_lens.stride(-1) == 1):
+        raise ValueError(f"{name}: contiguous metadata")
+    return True, T, Hq
 
 
 def _row_tiles(rows: int, head_dim: int) -> int:
@@ -271,14 +289,14 @@ ROW_LEAST = 4                 # units a part at least: one a wave
 ROW_LONG = 48                 # longer parts are halved
 
 
-def _launch_rows(q, out, cache, block_tables, seq_lens, cu, seqs, n, sequences, scale, causal, window, chunk, tiles, parts, per):
-    Hq, D = q.shape[1], q.shape[2]
+def _launch_rows(name, q, out, cache, block_tables, seq_lens, cu, seqs, n, sequences, scale, causal, window, chunk, tiles, parts, per):
+    _, Hq, D = q.shape
     ws = torch.empty(parts * cache.num_kv_heads * 16 * tiles * (D + 2) + 2 * sequences, dtype=torch.float32,
-                     device=q.device) if parts > n else None
-    check(lib().eia_quant_rows(
-        ptr(q), q.stride(0), ptr(out), out.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(seq_lens), cu, seqs, n,
-        float(scale), Hq, cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per,
-        ROW_LEAST, ROW_SHIFT, ptr(ws), stream(q)), "quant_rows")
+                     device=cache.device) if parts > n else None
+    _launch(name, lib().eia_quant_rows, cache.device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *cache._args,
+            block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu, seqs, n, float(scale), Hq,
+            cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, ROW_SHIFT,
+            ptr(ws))
 
 
 def _rows_per(units: int) -> int:
@@ -300,24 +318,25 @@ def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tenso
 
     Rows of length 0 become zeros.  Nothing is read back: lengths and tables may change under a captured graph, up to the
     tables' width."""
-    _check_attention("quant_decode", q, cache, block_tables, seq_lens, scale, out)
-    B, Hq, D = q.shape
-    require(block_tables.shape[0] >= B and seq_lens.numel() >= B, "quant_decode: metadata rows < batch")
-    if not (use_hip(q, cache.k) and q.dtype == torch.bfloat16):
+    B = q.shape[0]
+    hip, _, Hq = _check_attention("quant_decode", q, cache, block_tables, seq_lens, B, scale, out)
+    if not hip:
         rows = [_attend_plain(q[b:b + 1], cache, block_tables[b], int(seq_lens[b]), scale, True, sliding_window, chunk_size) for b in range(B)]
         r = torch.cat(rows).to(q.dtype) if B else q.clone()
         return r if out is None else out.copy_(r)
-    o = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
-    _check_hip("quant_decode", q, cache, o, block_tables, seq_lens)
-    tiles = _row_tiles(Hq // cache.num_kv_heads, D)
-    require(tiles > 0, "quant_decode: too many query heads a kv head")
+    o = torch.empty((B, Hq, cache.head_dim), dtype=torch.bfloat16, device=cache.device) if out is None else out
+    tiles = _row_tiles(Hq // cache.num_kv_heads, cache.head_dim)
+    if tiles == 0:
+        raise ValueError("quant_decode: too many query heads a kv head")
     if B == 0:
         return o
-    span = min(w for w in (block_tables.shape[1] * cache.block_size, sliding_window, chunk_size) if w)
-    units = -(-span // UNIT) + (1 if sliding_window or chunk_size else 0)
+    span = block_tables.shape[1] * cache.block_size
+    units = -(-span // UNIT)
+    for w in (sliding_window, chunk_size):
+        if w:
+            units = min(units, -(-w // UNIT) + 1)
     parts = _row_parts(B, units, cache.num_kv_heads)
-    with _launch_on(q):
-        _launch_rows(q, o, cache, block_tables, seq_lens, None, None, B, B, scale, True, sliding_window, chunk_size, tiles, parts, 0)
+    _launch_rows("quant_decode", q, o, cache, block_tables, seq_lens, None, None, B, B, scale, True, sliding_window, chunk_size, tiles, parts, 0)
     return o
 
 
@@ -340,6 +359,9 @@ class QuantPrefillPlan:
     row_tiles: int = 1
     row_parts: int = 1
     row_per: int = 0
+
+    def __post_init__(self):
+        self.tokens, self.longest = sum(self.q_lens), max(self.kv_lens, default=0)
 
 
 FLASH_ROWS = {64: 256, 128: 256, 256: 128}      # (query, head) rows of a workgroup of csrc/kernels/quant_flash.hip
@@ -400,7 +422,7 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
         items.sort(key=lambda b: -b[0])
         plan.n_items, plan.n_merge = len(items), len(merges) // 4
     flat = [x for _, it in items for x in it] + merges + few
-    plan.lists = torch.tensor(flat, dtype=torch.int32, device=device)
+    plan.lists = torch.tensor(flat, dtype=torch.int32, pin_memory=torch.device(device).type == "cuda").to(device, non_blocking=True)
     return plan
 
 
@@ -452,35 +474,62 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
     """q [T, Hq, D], chunks of new tokens at the end of their sequences (rows cu_q[s] .. cu_q[s + 1]), whose keys and values the
     cache already holds -> out [T, Hq, D] (``paged_prefill`` for the 8-bit cache).  ``plan`` holds the lengths on the host; rows
     that see no key become zeros."""
-    _check_attention("quant_prefill", q, cache, block_tables, seq_lens, scale, out)
-    T, Hq, D = q.shape
     n = len(plan.q_lens)
-    require((plan.num_heads, plan.num_kv_heads, plan.head_dim) == (Hq, cache.num_kv_heads, D), "quant_prefill: plan of other heads")
-    require(sum(plan.q_lens) == T and cu_q.numel() >= n + 1 and cu_q.dtype == torch.int32, "quant_prefill: plan of other chunks")
-    require(block_tables.shape[0] >= n and seq_lens.numel() >= n, "quant_prefill: metadata rows < sequences")
-    require(all(L <= block_tables.shape[1] * cache.block_size for L in plan.kv_lens), "quant_prefill: tables shorter than the sequences")
-    if not (use_hip(q, cache.k) and q.dtype == torch.bfloat16):
+    hip, T, Hq = _check_attention("quant_prefill", q, cache, block_tables, seq_lens, n, scale, out)
+    D = cache.head_dim
+    if not (plan.num_heads == Hq and plan.num_kv_heads == cache.num_kv_heads and plan.head_dim == D):
+        raise ValueError("quant_prefill: plan of other heads")
+    if not (plan.tokens == T and cu_q.numel() >= n + 1 and cu_q.dtype is torch.int32 and cu_q.stride(-1) == 1):
+        raise ValueError("quant_prefill: plan of other chunks")
+    if plan.longest > block_tables.shape[1] * cache.block_size:
+        raise ValueError("quant_prefill: tables shorter than the sequences")
+    if not hip:
         at, rows = 0, []
         for s, (m, L) in enumerate(zip(plan.q_lens, plan.kv_lens)):
             rows.append(_attend_plain(q[at:at + m], cache, block_tables[s], L, scale, plan.causal, plan.sliding_window, plan.chunk_size))
             at += m
         r = torch.cat(rows).to(q.dtype) if rows else q.clone()
         return r if out is None else out.copy_(r)
-    o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
-    _check_hip("quant_prefill", q, cache, o, block_tables, seq_lens, cu_q)
-    if plan.n_items + plan.n_rows == 0:
-        return o
-    require(plan.lists is not None and plan.lists.device == q.device, "quant_prefill: plan of another device")
-    base = plan.lists.data_ptr()
-    with _launch_on(q):
-        if plan.n_items:
-            ws = torch.empty(plan.slots * cache.num_kv_heads * FLASH_ROWS[D] * (D + 2), dtype=torch.float32, device=q.device) if plan.slots else None
-            check(lib().eia_quant_flash(
-                ptr(q), q.stride(0), ptr(o), o.stride(0), *cache._args, ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(seq_lens),
-                ptr(cu_q), base, plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq,
-                cache.num_kv_heads, D, cache.block_size, 1 if plan.causal else 0, plan.sliding_window or 0, plan.chunk_size or 0,
-                stream(q)), "quant_prefill")
-        if plan.n_rows:
-            _launch_rows(q, o, cache, block_tables, seq_lens, ptr(cu_q), base + 32 * plan.n_items + 16 * plan.n_merge, plan.n_rows, n, scale,
-                         plan.causal, plan.sliding_window, plan.chunk_size, plan.row_tiles, plan.row_parts, plan.row_per)
+    if not (plan.lists.device == cu_q.device == cache.device):
+        raise ValueError("quant_prefill: plan and chunks on the cache's device")
+    o = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=cache.device) if out is None else out
+    base, window, chunk = plan.lists.data_ptr(), plan.sliding_window or 0, plan.chunk_size or 0
+    if plan.n_items:
+        ws = torch.empty(plan.slots * cache.num_kv_heads * FLASH_ROWS[D] * (D + 2), dtype=torch.float32, device=cache.device) if plan.slots else None
+        _launch("quant_prefill", lib().eia_quant_flash, cache.device, q.data_ptr(), q.stride(0), o.data_ptr(), o.stride(0), *cache._args,
+                block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu_q.data_ptr(), base,
+                plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq, cache.num_kv_heads, D,
+                cache.block_size, 1 if plan.causal else 0, window, chunk)
+    if plan.n_rows:
+        _launch_rows("quant_prefill", q, o, cache, block_tables, seq_lens, cu_q.data_ptr(), base + 32 * plan.n_items + 16 * plan.n_merge,
+                     plan.n_rows, n, scale, plan.causal, window, chunk, plan.row_tiles, plan.row_parts, plan.row_per)
     return o
+
+
+def quant_attention(q: torch.Tensor, cache: QuantKVCache, md, scale: float, sliding_window: Optional[int] = None,
+                    chunk_size: Optional[int] = None) -> torch.Tensor:
+    """The step's decode and prefill parts (``attention.attention`` for the 8-bit cache). q [T, Hq, D]."""
+    nd = md.num_decode
+    out = None
+    if md.num_prefill_tokens:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        key = ("quant", q.shape[1], cache.num_kv_heads, cache.head_dim, sliding_window, chunk_size)
+        plan = md.work_cache.get(key)                # once a step: its layers are alike
+        if plan is None:
+            lens, cu = md.prefill_q_lens, md.prefill_cu_q
+            if lens is None:
+                cu = cu.tolist()
+                lens = [b - a for a, b in zip(cu, cu[1:])]
+            kv = md.prefill_kv_lens
+            if kv is None:
+                kv = md.prefill_seq_lens.tolist()
+            plan = quant_prefill_plan(lens, kv, q.shape[1], cache.num_kv_heads, cache.head_dim, q.device, md.causal, sliding_window,
+                                      chunk_size)
+            md.work_cache[key] = plan
+        quant_prefill(q[nd:], cache, md.prefill_block_tables, md.prefill_seq_lens, md.prefill_cu_q, plan, scale, out=out[nd:])
+    if nd:
+        part = None if out is None else out[:nd]
+        o = quant_decode(q if nd == q.shape[0] else q[:nd], cache, md.decode_block_tables, md.decode_seq_lens, scale, sliding_window,
+                         chunk_size, out=part)
+        out = o if out is None else out
+    return out if out is not None else torch.empty_like(q)

@@ -87,11 +87,13 @@ def attend64(q, parts, bt, q_lens, lens, scale, causal=True, window=0, chunk=0):
 
 
 def check_attention(got, want, mag):
-    """Weights are rounded to bf16 once (half a step, 2^-8 of each), the output once more (2^-8 of it); scores and sums are fp32
-    (2^-12 of the weighted magnitudes covers scores of some hundreds and thousands of terms).  A weight under 2^-126 of the largest becomes 0
-    in fp32: with at most 2^10 such keys here, of values under 2^7, that is less than 2^-109."""
+    """Weights w are rounded to bf16 once: w (1 + d), |d| <= 2^-8, half a step.  Their sum is that of the weights before or after
+    the rounding, a factor 1 + D, |D| <= 2^-8.  So out = sum w (1 + d) v / (sum w (1 + D)) is off by at most 2^-8 sum w |v| / sum w from the
+    first and 2^-8 |out| from the second, and the output's own rounding adds 2^-8 |out|.  Scores and sums are fp32 (2^-12 of the weighted
+    magnitudes covers scores of some hundreds and thousands of terms, and the products of the roundings).  A weight under 2^-126 of the
+    largest becomes 0 in fp32: with at most 2^10 such keys here, of values under 2^7, that is less than 2^-109."""
     got = got.double()
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     fine = ~torch.isnan(want)
-    off = (got - want).abs()[fine] - (2 ** -8 * (want.abs() + mag) + 2 ** -12 * mag + 2.0 ** -109)[fine]
+    off = (got - want).abs()[fine] - (2 ** -8 * (2 * want.abs() + mag) + 2 ** -12 * mag + 2.0 ** -109)[fine]
     assert off.numel() == 0 or float(off.max()) <= 0.0, float(off.max())

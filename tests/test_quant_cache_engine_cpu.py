@@ -1,0 +1,79 @@
+"""The engine over the 8-bit key/value cache (CPU): every model with the common cache, portions, prefix hits, swaps, and the
+command line."""
+
+import pytest
+import torch
+
+from enterprise_inference_amd.config import CacheConfig, EngineConfig, ModelConfig, SchedulerConfig
+from enterprise_inference_amd.engine.llm_engine import LLMEngine
+from enterprise_inference_amd.engine.sampling_params import SamplingParams
+from enterprise_inference_amd.models import catalog
+from enterprise_inference_amd.ops.quant_cache import QuantKVCache
+
+PROMPTS = [list(range(3 + i, 60 + 3 * i)) for i in range(4)] + [[7, 8, 9]]
+PARAMS = SamplingParams(max_tokens=12, temperature=0, ignore_eos=True)
+
+
+def _engine(d, mbt=64, blocks=64, swap_gb=0.0, prefix=False, dtype=torch.float8_e4m3fn):
+    cfg = EngineConfig(model=ModelConfig.from_hf_dict(d),
+                       cache=CacheConfig(block_size=16, num_gpu_blocks=blocks, swap_space_gb=swap_gb,
+                                         enable_prefix_caching=prefix, cache_dtype=dtype),
+                       scheduler=SchedulerConfig(max_num_seqs=8, max_num_batched_tokens=mbt, max_model_len=256),
+                       device="cpu", dtype=torch.float32, load_format="dummy")
+    return LLMEngine(cfg)
+
+
+def _tokens(eng, prompts=PROMPTS):
+    return [o.outputs[0].token_ids for o in eng.generate(prompt_token_ids=prompts, params=PARAMS)]
+
+
+def _config(arch):
+    if arch == "OPTForCausalLM":
+        return catalog.tiny_config(arch, hidden_size=256)
+    return catalog.tiny_config(arch, head_dim=64, **({"sliding_window": 24} if arch == "MistralForCausalLM" else {}))
+
+
+@pytest.mark.parametrize("arch", ["LlamaForCausalLM", "Qwen2ForCausalLM", "Qwen3ForCausalLM", "MistralForCausalLM", "MixtralForCausalLM",
+                                  "OPTForCausalLM"])
+def test_portions_give_the_tokens_of_whole_prompts(arch):
+    d = _config(arch)
+    whole = _engine(d, mbt=512)
+    kv = whole.executor.runner.kv_caches[0]
+    assert isinstance(kv, QuantKVCache)
+    assert whole.executor.runner.kv_block_bytes() * 4 < 1.1 * _engine(d, dtype=None).executor.runner.kv_block_bytes()
+    first = _tokens(whole)
+    assert all(len(t) == 12 for t in first)
+    assert _tokens(_engine(d, mbt=20)) == first
+
+
+def test_prefix_hits_and_swaps_keep_the_tokens(monkeypatch):
+    monkeypatch.setenv("EIA_CPU_SWAP", "1")
+    d = _config("LlamaForCausalLM")
+    prompts = [list(range(3 + i, 40 + i)) for i in range(6)]
+    first = _tokens(_engine(d, blocks=256), prompts)
+    tight = _engine(d, blocks=16, swap_gb=0.01)
+    assert _tokens(tight, prompts) == first and tight.scheduler.num_swapouts > 0
+    hits = _engine(d, prefix=True)
+    assert _tokens(hits, prompts[:1]) == first[:1]
+    again = hits.generate(prompt_token_ids=prompts[:1], params=PARAMS)
+    assert again[0].num_cached_tokens > 0 and again[0].outputs[0].token_ids == first[0]
+
+
+def test_what_is_refused():
+    with pytest.raises(ValueError, match="heads of 64"):
+        _engine(catalog.tiny_config())                       # heads of 32
+    cfg = ModelConfig.from_hf_dict(_config("LlamaForCausalLM"))
+    cfg.architecture = "Sekolorn"                            # lays out its own caches
+    with pytest.raises(ValueError, match="lay out their own"):
+        EngineConfig(model=cfg, cache=CacheConfig(cache_dtype=torch.float8_e4m3fn), device="cpu", dtype=torch.float32)
+
+
+def test_command_line(tmp_path):
+    import json
+
+    from enterprise_inference_amd.entrypoints.cli_args import engine_config_from_args, parse_args
+    (tmp_path / "config.json").write_text(json.dumps(_config("LlamaForCausalLM")))
+    base = ["--model", str(tmp_path), "--device", "cpu", "--load-format", "dummy"]
+    cfg = engine_config_from_args(parse_args(base + ["--kv-cache-dtype", "fp8_per_token_head"]))
+    assert cfg.cache.cache_dtype == torch.float8_e4m3fn
+    assert engine_config_from_args(parse_args(base)).cache.cache_dtype == torch.float32
