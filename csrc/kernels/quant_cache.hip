@@ -26,82 +26,89 @@ template <int D, bool NEOX> EIA_DEV void halves_of(int sub, int& e0, int& e1) {
   e1 = NEOX ? D / 2 + 8 * sub : 16 * sub + 8;
 }
 
-// Sixteen values of a head's row, with the bias.
-template <int D, bool NEOX>
-EIA_DEV void load_row(const QuantSrc& src, int t, int head, int ntot, int sub, float (&x)[16]) {
-  int e[2];
-  halves_of<D, NEOX>(sub, e[0], e[1]);
-  if (src.part) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = 0.f;
-    for (int k = 0; k < src.sk; ++k) {
-      const float* p = src.part + k * src.slab + ((long)t * ntot + head) * D;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(p + e[h] + 4 * q);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[8 * h + 4 * q + j] += v[j];
-        }
-    }
-  } else {
-    const bf16_t* p = src.qkv + (long)t * src.stride + (long)head * D;
+// Sixteen values of a head's row, with the bias: asked for, and taken.
+template <int D, bool NEOX> struct RowLoad {
+  bf16x8 v[2], b[2];
+  EIA_DEV void ask(const QuantSrc& src, int t, int head, int sub) {
+    int e[2];
+    halves_of<D, NEOX>(sub, e[0], e[1]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bf16x8 v = *reinterpret_cast<const bf16x8*>(p + e[h]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[8 * h + j] = bf2f(v[j]);
+      if (!src.part) v[h] = *reinterpret_cast<const bf16x8*>(src.qkv + (long)t * src.stride + (long)head * D + e[h]);
+      if (src.bias) b[h] = *reinterpret_cast<const bf16x8*>(src.bias + (long)head * D + e[h]);
     }
   }
-  if (src.bias) {
+  EIA_DEV void take(const QuantSrc& src, int t, int head, int ntot, int sub, float (&x)[16]) {
+    int e[2];
+    halves_of<D, NEOX>(sub, e[0], e[1]);
+    if (src.part) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bf16x8 v = *reinterpret_cast<const bf16x8*>(src.bias + (long)head * D + e[h]);
+      for (int j = 0; j < 16; ++j) x[j] = 0.f;
+      for (int k = 0; k < src.sk; ++k) {
+        const float* p = src.part + k * src.slab + ((long)t * ntot + head) * D;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[8 * h + j] += bf2f(v[j]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(p + e[h] + 4 * q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[8 * h + 4 * q + j] += y[j];
+          }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = bf2f(v[j / 8][j % 8]);
+    }
+    if (src.bias) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] += bf2f(b[j / 8][j % 8]);
     }
   }
-}
+};
 
-template <int D, bool NEOX>
-EIA_DEV void norm_row(const bf16_t* w, float eps, int sub, float (&x)[16]) {
-  float ss = 0.f;
+// T: queries are rounded to bf16 and formed in fp32; keys in fp64 (their codes are borders apart, and the heads are few): what
+// a code is the nearest to is then off by fp32's last rounding alone.
+template <int D, bool NEOX, typename T>
+EIA_DEV void norm_row(const bf16_t* w, float eps, int sub, T (&x)[16]) {
+  T ss = 0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) ss += x[j] * x[j];
 #pragma unroll
   for (int o = 1; o < D / 16; o <<= 1) ss += __shfl_xor(ss, o, 64);
-  const float inv = 1.f / sqrtf(ss / (float)D + eps);
+  const T inv = (T)1 / sqrt(ss / (T)D + (T)eps);
   int e[2];
   halves_of<D, NEOX>(sub, e[0], e[1]);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const bf16x8 v = *reinterpret_cast<const bf16x8*>(w + e[h]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[8 * h + j] *= inv * bf2f(v[j]);
+    for (int j = 0; j < 8; ++j) x[8 * h + j] *= inv * (T)bf2f(v[j]);
   }
 }
 
-// cs: cos [D / 2] | sin [D / 2] of the token's position.
-template <int D, bool NEOX>
-EIA_DEV void rotate_row(const float* cs, int sub, float (&x)[16]) {
+// A token's cos and sin for a lane's eight pairs: cs is cos [D / 2] | sin [D / 2].
+template <int D> struct Turn {
   float c[8], s[8];
+  EIA_DEV void ask(const float* cs, int sub) {
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(cs + 8 * sub + 4 * q), b = *reinterpret_cast<const f32x4*>(cs + D / 2 + 8 * sub + 4 * q);
+    for (int q = 0; q < 2; ++q) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(cs + 8 * sub + 4 * q), b = *reinterpret_cast<const f32x4*>(cs + D / 2 + 8 * sub + 4 * q);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[4 * q + j] = a[j], s[4 * q + j] = b[j];
+      for (int j = 0; j < 4; ++j) c[4 * q + j] = a[j], s[4 * q + j] = b[j];
+    }
   }
+  template <bool NEOX, typename T> EIA_DEV void rotate(T (&x)[16]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float &a = x[NEOX ? j : 2 * j], &b = x[NEOX ? 8 + j : 2 * j + 1];
-    const float ra = fmaf(a, c[j], -(b * s[j])), rb = fmaf(b, c[j], a * s[j]);
-    a = ra;
-    b = rb;
+    for (int j = 0; j < 8; ++j) {
+      T &a = x[NEOX ? j : 2 * j], &b = x[NEOX ? 8 + j : 2 * j + 1];
+      const T ra = fma(a, (T)c[j], -(b * (T)s[j])), rb = fma(b, (T)c[j], a * (T)s[j]);
+      a = ra;
+      b = rb;
+    }
   }
-}
+};
 
-template <int D, bool NEOX, int TT>
+template <int D, bool NEOX, int TT, int NH>
 __global__ void __launch_bounds__(256)
 quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float* __restrict__ cos_sin,
                    const int* __restrict__ slots, QuantCache cache, long num_slots, bf16_t* __restrict__ q_out, int T, int Hq,
@@ -113,18 +120,28 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
   int e0, e1;
   halves_of<D, NEOX>(sub, e0, e1);
   if ((int)blockIdx.y < q_groups) {
-    const int h = blockIdx.y * HPB + at / TT;
-    if (t >= T || h >= Hq) return;                         // (a head's lanes together)
-    float x[16];
-    load_row<D, NEOX>(src, t, h, ntot, sub, x);
-    if (src.q_norm) norm_row<D, NEOX>(src.q_norm, src.eps, sub, x);
-    if (cos_sin) rotate_row<D, NEOX>(cos_sin + (long)positions[t] * D, sub, x);
-    bf16x8 a, b;
+    const int h0 = blockIdx.y * HPB * NH + at / TT;        // heads h0, h0 + HPB, ...: one token's angles for all of them
+    if (t >= T || h0 >= Hq) return;                        // (a head's lanes together)
+    RowLoad<D, NEOX> row[NH];
+    Turn<D> turn;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = f2bf(x[j]), b[j] = f2bf(x[8 + j]);
-    bf16_t* o = q_out + ((long)t * Hq + h) * D;
-    *reinterpret_cast<bf16x8*>(o + e0) = a;
-    *reinterpret_cast<bf16x8*>(o + e1) = b;
+    for (int n = 0; n < NH; ++n) row[n].ask(src, t, min(h0 + n * HPB, Hq - 1), sub);
+    if (cos_sin) turn.ask(cos_sin + (long)positions[t] * D, sub);
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const int h = h0 + n * HPB;
+      if (h >= Hq) break;
+      float x[16];
+      row[n].take(src, t, h, ntot, sub, x);
+      if (src.q_norm) norm_row<D, NEOX>(src.q_norm, src.eps, sub, x);
+      if (cos_sin) turn.template rotate<NEOX>(x);
+      bf16x8 a, b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = f2bf(x[j]), b[j] = f2bf(x[8 + j]);
+      bf16_t* o = q_out + ((long)t * Hq + h) * D;
+      *reinterpret_cast<bf16x8*>(o + e0) = a;
+      *reinterpret_cast<bf16x8*>(o + e1) = b;
+    }
     return;
   }
   __shared__ __align__(16) uint8_t tile[HPB][D][TT];
@@ -133,10 +150,22 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
   const bool live = slot >= 0 && slot < num_slots && h < Hkv;
   if (live) {
     float k[16], v[16];
-    load_row<D, NEOX>(src, t, Hq + h, ntot, sub, k);
-    load_row<D, NEOX>(src, t, Hq + Hkv + h, ntot, sub, v);
-    if (src.k_norm) norm_row<D, NEOX>(src.k_norm, src.eps, sub, k);
-    if (cos_sin) rotate_row<D, NEOX>(cos_sin + (long)positions[t] * D, sub, k);
+    RowLoad<D, NEOX> krow, vrow;
+    Turn<D> turn;
+    krow.ask(src, t, Hq + h, sub);
+    vrow.ask(src, t, Hq + Hkv + h, sub);
+    if (cos_sin) turn.ask(cos_sin + (long)positions[t] * D, sub);
+    krow.take(src, t, Hq + h, ntot, sub, k);
+    vrow.take(src, t, Hq + Hkv + h, ntot, sub, v);
+    if (src.k_norm || cos_sin) {
+      double x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = k[j];
+      if (src.k_norm) norm_row<D, NEOX>(src.k_norm, src.eps, sub, x);
+      if (cos_sin) turn.template rotate<NEOX>(x);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) k[j] = (float)x[j];
+    }
     // magnitudes as bits: what is not finite is the largest
     unsigned mk = 0, mv = 0;
 #pragma unroll
@@ -257,17 +286,17 @@ EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part,
   const QuantSrc src{(const bf16_t*)qkv, part, qkv_stride, (long)T * (Hq + 2 * Hkv) * D, sk, (const bf16_t*)bias, (const bf16_t*)q_norm,
                      (const bf16_t*)k_norm, eps};
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
-#define QW_GO(D, NX, TT)                                                                                                          \
+#define QW_GO(D, NX, TT, NH)                                                                                                      \
   do {                                                                                                                            \
     constexpr int hpb = 256 / (D / 16) / TT;                                                                                      \
-    const int qg = (Hq + hpb - 1) / hpb;                                                                                          \
-    hipLaunchKernelGGL((quant_write_kernel<D, NX, TT>), dim3((T + TT - 1) / TT, qg + (Hkv + hpb - 1) / hpb), dim3(256), 0, st, src, \
+    const int qg = (Hq + hpb * NH - 1) / (hpb * NH);                                                                              \
+    hipLaunchKernelGGL((quant_write_kernel<D, NX, TT, NH>), dim3((T + TT - 1) / TT, qg + (Hkv + hpb - 1) / hpb), dim3(256), 0, st, src, \
                        positions, cos_sin, slots, c, (long)pages * bs, (bf16_t*)q_out, T, Hq, qg);                                \
   } while (0)
 #define QW_D(D)                                                                                          \
   do {                                                                                                   \
-    if (T >= 256) { if (neox) QW_GO(D, true, 16); else QW_GO(D, false, 16); }                            \
-    else { if (neox) QW_GO(D, true, 1); else QW_GO(D, false, 1); }                                       \
+    if (T >= 256) { if (neox) QW_GO(D, true, 16, 4); else QW_GO(D, false, 16, 4); }                      \
+    else { if (neox) QW_GO(D, true, 1, 1); else QW_GO(D, false, 1, 1); }                                 \
   } while (0)
   switch (D) {
     case 64: QW_D(64); break;
