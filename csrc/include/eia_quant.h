@@ -27,6 +27,13 @@ struct QuantCache {
   EIA_DEV uint8_t* vscale(int page, int h, int off) const { return vs + page * scales + (long)h * bs + off; }
 };
 
+// 16 bytes that are read once and leave nothing in the caches, or as usual.
+template <bool ONCE> EIA_DEV uint4 quant_load(const void* p) {
+  typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+  if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+  return *reinterpret_cast<const uint4*>(p);
+}
+
 // Byte of a row whose largest magnitude has these bits (a row that is not finite: 0x7f800000 or more, not asked here).
 // 448 = 1.75 * 2^8: a mantissa over 1.75 carries into the exponent.
 EIA_DEV unsigned quant_byte(unsigned amax_bits) {

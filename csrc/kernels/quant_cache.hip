@@ -27,14 +27,14 @@ template <int D, bool NEOX> EIA_DEV void halves_of(int sub, int& e0, int& e1) {
 }
 
 // Sixteen values of a head's row, with the bias: asked for, and taken.
-template <int D, bool NEOX> struct RowLoad {
+template <int D, bool NEOX, bool ONCE> struct RowLoad {
   bf16x8 v[2], b[2];
   EIA_DEV void ask(const QuantSrc& src, int t, int head, int sub) {
     int e[2];
     halves_of<D, NEOX>(sub, e[0], e[1]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (!src.part) v[h] = *reinterpret_cast<const bf16x8*>(src.qkv + (long)t * src.stride + (long)head * D + e[h]);
+      if (!src.part) v[h] = __builtin_bit_cast(bf16x8, quant_load<ONCE>(src.qkv + (long)t * src.stride + (long)head * D + e[h]));
       if (src.bias) b[h] = *reinterpret_cast<const bf16x8*>(src.bias + (long)head * D + e[h]);
     }
   }
@@ -108,7 +108,7 @@ template <int D> struct Turn {
   }
 };
 
-template <int D, bool NEOX, int TT, int NH>
+template <int D, bool NEOX, int TT, int NH, bool ONCE>
 __global__ void __launch_bounds__(256)
 quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float* __restrict__ cos_sin,
                    const int* __restrict__ slots, QuantCache cache, long num_slots, bf16_t* __restrict__ q_out, int T, int Hq,
@@ -122,7 +122,7 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
   if ((int)blockIdx.y < q_groups) {
     const int h0 = blockIdx.y * HPB * NH + at / TT;        // heads h0, h0 + HPB, ...: one token's angles for all of them
     if (t >= T || h0 >= Hq) return;                        // (a head's lanes together)
-    RowLoad<D, NEOX> row[NH];
+    RowLoad<D, NEOX, ONCE> row[NH];
     Turn<D> turn;
 #pragma unroll
     for (int n = 0; n < NH; ++n) row[n].ask(src, t, min(h0 + n * HPB, Hq - 1), sub);
@@ -150,7 +150,7 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
   const bool live = slot >= 0 && slot < num_slots && h < Hkv;
   if (live) {
     float k[16], v[16];
-    RowLoad<D, NEOX> krow, vrow;
+    RowLoad<D, NEOX, ONCE> krow, vrow;
     Turn<D> turn;
     krow.ask(src, t, Hq + h, sub);
     vrow.ask(src, t, Hq + Hkv + h, sub);
@@ -228,7 +228,7 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
 
 // Rows of sixteen slots and one head a workgroup part: keys straight through, values through LDS as the cache holds them.
 // Rows of slots outside the cache are zeros.
-template <int D>
+template <int D, bool ONCE>
 __global__ void __launch_bounds__(256)
 quant_read_kernel(QuantCache cache, const int* __restrict__ slots, long num_slots, int n, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out) {
   constexpr int TPH = D / 16, HPB = 256 / TPH / QUANT_GROUP;
@@ -242,7 +242,7 @@ quant_read_kernel(QuantCache cache, const int* __restrict__ slots, long num_slot
     const int page = first / cache.bs, off = first % cache.bs;
     for (int r = threadIdx.x; r < HPB * D; r += 256)
       if (h0 + r / D < Hkv)
-        *reinterpret_cast<uint4*>(&tile[r / D][QUANT_GROUP * (r % D)]) = *reinterpret_cast<const uint4*>(cache.values(page, h0 + r / D, off, D) + QUANT_GROUP * (r % D));
+        *reinterpret_cast<uint4*>(&tile[r / D][QUANT_GROUP * (r % D)]) = quant_load<ONCE>(cache.values(page, h0 + r / D, off, D) + QUANT_GROUP * (r % D));
   } else {
     const int page = there ? mine / cache.bs : 0, off = there ? mine % cache.bs : 0;
     for (int r = threadIdx.x / 16; r < HPB * D; r += 16)
@@ -256,7 +256,7 @@ quant_read_kernel(QuantCache cache, const int* __restrict__ slots, long num_slot
   const bool live = slot >= 0 && slot < num_slots;
   const int page = live ? (int)(slot / cache.bs) : 0, off = live ? (int)(slot % cache.bs) : 0;
   const unsigned bk = live ? *cache.kscale(page, h, off) : 127, bv = live ? *cache.vscale(page, h, off) : 127;
-  uint4 w = live ? *reinterpret_cast<const uint4*>(cache.key(page, h, off, D) + 16 * sub) : make_uint4(0, 0, 0, 0), u;
+  uint4 w = live ? quant_load<ONCE>(cache.key(page, h, off, D) + 16 * sub) : make_uint4(0, 0, 0, 0), u;
   unsigned x[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -286,18 +286,24 @@ EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part,
   const QuantSrc src{(const bf16_t*)qkv, part, qkv_stride, (long)T * (Hq + 2 * Hkv) * D, sk, (const bf16_t*)bias, (const bf16_t*)q_norm,
                      (const bf16_t*)k_norm, eps};
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
-#define QW_GO(D, NX, TT, NH)                                                                                                      \
+#define QW_GO(D, NX, TT, NH, ONCE)                                                                                                      \
   do {                                                                                                                            \
     constexpr int hpb = 256 / (D / 16) / TT;                                                                                      \
     const int qg = (Hq + hpb * NH - 1) / (hpb * NH);                                                                              \
-    hipLaunchKernelGGL((quant_write_kernel<D, NX, TT, NH>), dim3((T + TT - 1) / TT, qg + (Hkv + hpb - 1) / hpb), dim3(256), 0, st, src, \
+    hipLaunchKernelGGL((quant_write_kernel<D, NX, TT, NH, ONCE>), dim3((T + TT - 1) / TT, qg + (Hkv + hpb - 1) / hpb), dim3(256), 0, st, src, \
                        positions, cos_sin, slots, c, (long)pages * bs, (bf16_t*)q_out, T, Hq, qg);                                \
   } while (0)
-#define QW_D(D)                                                                                          \
-  do {                                                                                                   \
-    if (T >= 256) { if (neox) QW_GO(D, true, 16, 4); else QW_GO(D, false, 16, 4); }                      \
-    else { if (neox) QW_GO(D, true, 1, 1); else QW_GO(D, false, 1, 1); }                                 \
+#define QW_N(D, NX)                                    \
+  do {                                                 \
+    if (T < 256) QW_GO(D, NX, 1, 1, false);            \
+    else if (once) QW_GO(D, NX, 16, 4, true);          \
+    else QW_GO(D, NX, 16, 4, false);                   \
   } while (0)
+#define QW_D(D) do { if (neox) QW_N(D, true); else QW_N(D, false); } while (0)
+  // Rows of more than a quarter of the last cache (256 MB) are read past the caches.  32 heads on 8 of 128, us as usual / past them: 4096
+  // tokens (48 MiB) 20.4 / 21.0, 8192 46.1 / 39.3, 32768 184 / 172; 12 on 4 of 256, 8192 (80 MiB) 37.7 / 33.2; 12 of 64, 8192 (36 MiB) 15.8 /
+  // 19.0.  Fewer than 256 tokens spread a token a workgroup row: sixteen together would leave the chip empty.
+  const bool once = (long)T * (Hq + 2 * Hkv) * D * 2 > 64l << 20;
   switch (D) {
     case 64: QW_D(64); break;
     case 128: QW_D(128); break;
@@ -305,6 +311,7 @@ EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part,
     default: return EIA_UNSUPPORTED;
   }
 #undef QW_D
+#undef QW_N
 #undef QW_GO
   EIA_LAUNCH_CHECK();
 }
@@ -314,11 +321,14 @@ EIA_API int eia_quant_read(const void* k, const void* v, const void* ks, const v
   if (n < 0 || Hkv <= 0 || bs <= 0 || bs % QUANT_GROUP) return EIA_BAD_SHAPE;
   if (n == 0) return EIA_OK;
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
+  // As the write's: us as usual / past the caches, 8 heads of 128: 4096 rows (8 MiB) 8.5 / 8.7, 8192 11.9 / 13.7, 32768 (64 MiB) 46.9 / 39.9.
+  const bool once = (long)n * Hkv * D * 2 > 32l << 20;
 #define QR_GO(D)                                                                                                                   \
   do {                                                                                                                             \
     constexpr int hpb = 256 / (D / 16) / QUANT_GROUP;                                                                              \
-    hipLaunchKernelGGL(quant_read_kernel<D>, dim3((n + QUANT_GROUP - 1) / QUANT_GROUP, (Hkv + hpb - 1) / hpb), dim3(256), 0, st, c, \
-                       slots, (long)pages * bs, n, (bf16_t*)k_out, (bf16_t*)v_out);                                                \
+    auto* f = once ? quant_read_kernel<D, true> : quant_read_kernel<D, false>;                                                     \
+    hipLaunchKernelGGL(f, dim3((n + QUANT_GROUP - 1) / QUANT_GROUP, (Hkv + hpb - 1) / hpb), dim3(256), 0, st, c, slots,            \
+                       (long)pages * bs, n, (bf16_t*)k_out, (bf16_t*)v_out);                                                       \
   } while (0)
   switch (D) {
     case 64: QR_GO(64); break;

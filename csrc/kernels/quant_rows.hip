@@ -19,13 +19,6 @@
 
 namespace {
 
-// Codes are read once, by one workgroup: they pass the caches by (8 kv heads, 32 rows of up to 16384 keys 164 -> 151 us, 64 of 2048
-// 52.4 -> 47.3).
-EIA_DEV uint4 once(const uint8_t* p) {
-  typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
-}
-
 constexpr int RU = 64;               // keys a wave takes at a time
 constexpr int RW = 4;                // waves of a workgroup
 
@@ -207,6 +200,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
     }
     return x;
   };
+  // codes are read once, by one workgroup: past the caches (8 kv heads, 32 rows of 8192 to 16384 keys 164 -> 151 us, 64 of 2048 52.4 -> 47.3)
   uint4 k[4][KC], ks, v[DT], vs;
   auto load_keys = [&](const Place& x) {
     const int page = UNI ? __builtin_amdgcn_readfirstlane(x.pk) : x.pk;
@@ -214,7 +208,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < KC; ++i) k[j][i] = once(p + 4 * j * D + 64 * i);
+      for (int i = 0; i < KC; ++i) k[j][i] = quant_load<true>(p + 4 * j * D + 64 * i);
     ks = *reinterpret_cast<const uint4*>(cache.kscale(page, kvh, x.ok) + (UNI ? 16 * (c >> 2) : 0));
   };
   auto load_values = [&](const Place& x) {
@@ -222,7 +216,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
     const uint8_t* p = cache.values(page, kvh, x.ov, D) + (UNI ? 16 * g * D : 0) + 16 * c;
     vs = *reinterpret_cast<const uint4*>(cache.vscale(page, kvh, x.ov) + (UNI ? 16 * g : 0));
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) v[dt] = once(p + 256 * dt);
+    for (int dt = 0; dt < DT; ++dt) v[dt] = quant_load<true>(p + 256 * dt);
   };
   Place next;
   auto compute = [&](int u, bool more) {

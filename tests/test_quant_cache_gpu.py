@@ -340,3 +340,26 @@ def test_what_is_refused_on_the_gpu():
         Q.rope_qkv_quant(torch.zeros(2, 6 * 128 + 4, dtype=BF, device="cuda")[:, :768], None, None, lens, cache, 4, 1, 128)
     with pytest.raises(ValueError):
         Q.quant_read(cache, lens.cpu())
+
+
+def test_large_writes_and_reads():
+    """Rows that are read past the caches: the same bytes as in portions that are not."""
+    Q = _q()
+    from enterprise_inference_amd.ops.rotary import RotaryCache
+    H, hk, D, bs, T = 32, 8, 128, 128, 5600                              # 65.6 MiB of rows
+    g = torch.Generator(device="cuda").manual_seed(21)
+    qkv = torch.randn(T, (H + 2 * hk) * D, generator=g, device="cuda").to(BF)
+    rot = RotaryCache(D, T, 10000.0, None, torch.device("cuda"))
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    a, b = (Q.QuantKVCache.allocate(44, hk, bs, D, "cuda") for _ in range(2))
+    q = Q.rope_qkv_quant(qkv, pos, rot, pos, a, H, hk, D)
+    parts = [Q.rope_qkv_quant(qkv[s], pos[s], rot, pos[s], b, H, hk, D) for s in (slice(0, 2800), slice(2800, 5500), slice(5500, T))]
+    assert torch.equal(q, torch.cat(parts))
+    for name in ("k", "v"):
+        assert torch.equal(getattr(a, name).view(torch.uint8), getattr(b, name).view(torch.uint8))
+    assert torch.equal(a.k_scale, b.k_scale) and torch.equal(a.v_scale, b.v_scale)
+    slots = torch.randint(0, T, (17000,), generator=g, device="cuda").to(torch.int32)       # 33 MiB of codes
+    slots[100:8000] = torch.arange(7900 - 5000, 7900 - 5000 + 7900, device="cuda").clamp(max=T - 1).to(torch.int32)
+    whole, half = Q.quant_read(a, slots), [Q.quant_read(a, slots[:8000]), Q.quant_read(a, slots[8000:])]
+    for i in range(2):
+        assert torch.equal(whole[i], torch.cat([h[i] for h in half]))
