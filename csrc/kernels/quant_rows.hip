@@ -37,6 +37,19 @@ struct Rows {
   unsigned magic;                    // 2^32 / groups, rounded up
 };
 
+// Sums of the lanes up to each one, by lane moves in registers (over LDS they take the wave six round trips).
+EIA_DEV int lanes_upto(int v) {
+#define UPTO(move, rows) v += __builtin_amdgcn_update_dpp(0, v, move, rows, 0xf, true)
+  UPTO(0x111, 0xf);                  // within sixteen lanes: from 1, 2, 4 and 8 below
+  UPTO(0x112, 0xf);
+  UPTO(0x114, 0xf);
+  UPTO(0x118, 0xf);
+  UPTO(0x142, 0xa);                  // the last of sixteen into the next sixteen (rows 1 and 3)
+  UPTO(0x143, 0xc);                  // the last of 32 into the upper 32
+#undef UPTO
+  return v;
+}
+
 struct Span { int lo, units; };      // first unit, units
 
 EIA_DEV Span rows_span(const Rows& r, int L, int qlen) {
@@ -80,9 +93,7 @@ EIA_DEV Part rows_part(const Rows& r, int Hkv, int y) {
       if (i != lane) length(i, s1, L1, q1, n1);
       sum += rows_span(r, L1, n1).units;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    per = rows_per(r, (long)sum * Hkv);
+    per = rows_per(r, (long)__builtin_amdgcn_readlane(lanes_upto(sum), 63) * Hkv);
   }
   const float inv = 1.f / (float)per;
   Part found{-1, 0, 0, 0, 0, 0, 0, {0, 0}};
@@ -93,12 +104,7 @@ EIA_DEV Part rows_part(const Rows& r, int Hkv, int y) {
     parts += parts * per < span.units;
     parts -= (parts - 1) * per >= span.units;
     parts = i0 + lane < r.n ? max(parts, 1) : 0;
-    int upto = parts;                                       // inclusive sums over the lanes
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, 64);
-      upto += lane >= o ? x : 0;
-    }
+    const int upto = lanes_upto(parts);
     const int at = y - before;
     const unsigned long long mine = __ballot(at >= upto - parts && at < upto);
     if (mine) {
