@@ -29,14 +29,16 @@ template <int D> struct Shape {
   static constexpr int BUF = FK * KS + D * VS;
 };
 
-struct Item { int seq, row, lo, tiles, slot, pad[3]; };    // row block, first key, key tiles, place of a part's sums (-1: whole)
-struct Merge { int seq, row, slot, parts; };
+// A block of rows of a sequence (its first query, queries and keys): first row, first key, key tiles, place of a part's sums (-1:
+// whole).  All that a workgroup would wait for one load after the other.
+struct Item { int seq, row, lo, tiles, slot, qbeg, qlen, len; };
+struct Merge { int row, slot, parts, qbeg, qlen, pad[3]; };
 
 struct Chunk {
   const bf16_t* q;
   bf16_t* out;
   long q_stride, out_stride;
-  const int *tables, *lens, *cu;
+  const int* tables;
   int bt_stride, Hq, causal, window, chunk;
   float scale_log2;
   f32x4* po;                         // sums of a part as its lanes hold them [slot][kv head][wave][D / 8][64]
@@ -81,7 +83,7 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r32 = lane & 31, h = lane >> 5;
   const Item it = items[blockIdx.y];
   const int kvh = blockIdx.x, Hkv = cache.Hkv, G = a.Hq / Hkv;
-  const int qbeg = a.cu[it.seq], qlen = a.cu[it.seq + 1] - qbeg, L = min(a.lens[it.seq], a.longest), ctx = L - qlen;
+  const int qbeg = it.qbeg, qlen = it.qlen, L = min(it.len, a.longest), ctx = L - qlen;
   const int rows = qlen * G, row0 = it.row + 32 * w;
   const bool window = a.window > 0 || a.chunk > 0;
   const int row = min(row0 + r32, rows - 1), qi = row / G;
@@ -348,7 +350,7 @@ quant_flash_merge_kernel(Chunk a, int Hkv, const Merge* __restrict__ merges) {
   constexpr int W = Shape<D>::THREADS / 64;
   const Merge it = merges[blockIdx.z];
   const int kvh = blockIdx.x, w = blockIdx.y, lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5, G = a.Hq / Hkv;
-  const int qbeg = a.cu[it.seq], rows = (a.cu[it.seq + 1] - qbeg) * G, row0 = it.row + 32 * w;
+  const int qbeg = it.qbeg, rows = it.qlen * G, row0 = it.row + 32 * w;
   if (row0 >= rows) return;
   const long step = (long)Hkv * W, at = ((long)it.slot * Hkv + kvh) * W + w;
   const float2* ml = a.ml + at * 32 + r32;
@@ -399,11 +401,10 @@ EIA_API int eia_quant_flash_rows(int D) {
   return D == 64 ? Shape<64>::ROWS : D == 128 ? Shape<128>::ROWS : D == 256 ? Shape<256>::ROWS : 0;
 }
 
-// items: n of {sequence, first row, first key, key tiles, slot or -1, 3 unused}; merges: n_merge of {sequence, first row, first slot,
-// parts}; ws: slots * Hkv * rows of a block * (D + 2) floats.
+// items: n of {sequence, first row, first key, key tiles, slot or -1, first query, queries, keys}; merges: n_merge of {first row, first
+// slot, parts, first query, queries, 3 unused}; ws: slots * Hkv * rows of a block * (D + 2) floats.
 EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
-                            const void* vs, long codes, long scales, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
-                            const int* items, int n, const int* merges, int n_merge, int slots, float* ws, float scale, int Hq, int Hkv,
+                            const void* vs, long codes, long scales, const int* tables, int bt_stride, int width, const int* items, int n, const int* merges, int n_merge, int slots, float* ws, float scale, int Hq, int Hkv,
                             int D, int bs, int causal, int window, int chunk, hipStream_t st) {
   if (n < 0 || n_merge < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || n > 65535 || n_merge > 65535 ||
       (slots > 0 && !ws))
@@ -411,7 +412,7 @@ EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_st
   if (n == 0) return EIA_OK;
   const int groups = bs / QUANT_GROUP, block = eia_quant_flash_rows(D);
   if (!block) return EIA_UNSUPPORTED;
-  const Chunk a{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, bt_stride, Hq, causal, window, chunk,
+  const Chunk a{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, bt_stride, Hq, causal, window, chunk,
                 scale * FLASH_LOG2E, reinterpret_cast<f32x4*>(ws), reinterpret_cast<float2*>(ws + (long)slots * Hkv * block * D), groups,
                 (int)std::min<long>((long)width * bs, INT_MAX),
                 (unsigned)(((1ull << 32) + groups - 1) / groups)};

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import dataclasses
 import heapq
+import itertools
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -351,7 +352,7 @@ class QuantPrefillPlan:
     causal: bool
     sliding_window: Optional[int]
     chunk_size: Optional[int]
-    lists: Optional[torch.Tensor]          # int32: blocks of 8, merges of 4, sequences of few rows
+    lists: Optional[torch.Tensor]          # int32: blocks of 8, merges of 8, sequences of few rows
     n_items: int = 0
     n_merge: int = 0
     slots: int = 0
@@ -383,7 +384,7 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
     require(num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim in HEAD_DIMS, "quant_prefill_plan: heads")
     plan = QuantPrefillPlan(q_lens, kv_lens, num_heads, num_kv_heads, head_dim, causal, sliding_window, chunk_size, None)
     G = num_heads // num_kv_heads
-    few, blocks = [], []
+    few, blocks, first = [], [], [0, *itertools.accumulate(q_lens)]
     R = FLASH_ROWS[head_dim]
     units = []
     for s, (n, L) in enumerate(zip(q_lens, kv_lens)):
@@ -395,9 +396,9 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
             units.append(-(-L // UNIT) - _first_key(max(L - n, 0), sliding_window, chunk_size) // UNIT if L else 0)
             continue
         for r in range(0, n * G, R):
-            first, last = L - n + r // G, L - n + (min(r + R, n * G) - 1) // G
-            hi = min(L, last + 1) if causal else L
-            lo = _first_key(first, sliding_window, chunk_size) // UNIT * UNIT
+            a, b = L - n + r // G, L - n + (min(r + R, n * G) - 1) // G          # positions of the block's first and last query
+            hi = min(L, b + 1) if causal else L
+            lo = _first_key(a, sliding_window, chunk_size) // UNIT * UNIT
             blocks.append((max(0, -(-(hi - lo) // UNIT)), s, r, lo))
     if few:
         plan.n_rows = len(few)
@@ -410,17 +411,17 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
         for tiles, s, r, lo in blocks:
             parts = max(1, -(-tiles // per))
             if parts == 1:
-                items.append((tiles, (s, r, lo, tiles, -1, 0, 0, 0)))
+                items.append((tiles, (s, r, lo, tiles, -1, first[s], q_lens[s], kv_lens[s])))
                 continue
             each = -(-tiles // parts)
             parts = -(-tiles // each)
-            merges += [s, r, plan.slots, parts]
+            merges += [r, plan.slots, parts, first[s], q_lens[s], 0, 0, 0]
             for p in range(parts):
                 t = min(each, tiles - p * each)
-                items.append((t, (s, r, lo + p * each * UNIT, t, plan.slots + p, 0, 0, 0)))
+                items.append((t, (s, r, lo + p * each * UNIT, t, plan.slots + p, first[s], q_lens[s], kv_lens[s])))
             plan.slots += parts
         items.sort(key=lambda b: -b[0])
-        plan.n_items, plan.n_merge = len(items), len(merges) // 4
+        plan.n_items, plan.n_merge = len(items), len(merges) // 8
     flat = [x for _, it in items for x in it] + merges + few
     plan.lists = torch.tensor(flat, dtype=torch.int32, pin_memory=torch.device(device).type == "cuda").to(device, non_blocking=True)
     return plan
@@ -472,8 +473,8 @@ def _flash_per(tiles: List[int], num_kv_heads: int, head_dim: int) -> int:
 def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor,
                   plan: QuantPrefillPlan, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, Hq, D], chunks of new tokens at the end of their sequences (rows cu_q[s] .. cu_q[s + 1]), whose keys and values the
-    cache already holds -> out [T, Hq, D] (``paged_prefill`` for the 8-bit cache).  ``plan`` holds the lengths on the host; rows
-    that see no key become zeros."""
+    cache already holds -> out [T, Hq, D] (``paged_prefill`` for the 8-bit cache).  ``plan`` holds the lengths that ``cu_q`` and
+    ``seq_lens`` hold on the device; rows that see no key become zeros."""
     n = len(plan.q_lens)
     hip, T, Hq = _check_attention("quant_prefill", q, cache, block_tables, seq_lens, n, scale, out)
     D = cache.head_dim
@@ -497,11 +498,10 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
     if plan.n_items:
         ws = torch.empty(plan.slots * cache.num_kv_heads * FLASH_ROWS[D] * (D + 2), dtype=torch.float32, device=cache.device) if plan.slots else None
         _launch("quant_prefill", lib().eia_quant_flash, cache.device, q.data_ptr(), q.stride(0), o.data_ptr(), o.stride(0), *cache._args,
-                block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu_q.data_ptr(), base,
-                plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq, cache.num_kv_heads, D,
+                block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], base, plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq, cache.num_kv_heads, D,
                 cache.block_size, 1 if plan.causal else 0, window, chunk)
     if plan.n_rows:
-        _launch_rows("quant_prefill", q, o, cache, block_tables, seq_lens, cu_q.data_ptr(), base + 32 * plan.n_items + 16 * plan.n_merge,
+        _launch_rows("quant_prefill", q, o, cache, block_tables, seq_lens, cu_q.data_ptr(), base + 32 * (plan.n_items + plan.n_merge),
                      plan.n_rows, n, scale, plan.causal, window, chunk, plan.row_tiles, plan.row_parts, plan.row_per)
     return o
 

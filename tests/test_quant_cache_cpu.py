@@ -138,13 +138,17 @@ def test_work_lists(heads, hk, d, q_lens, lens, causal, window):
     flat, G, R = plan.lists.tolist(), heads // hk, 128 if d == 256 else 256
     items = [flat[8 * i:8 * i + 5] for i in range(plan.n_items)]
     at = 8 * plan.n_items
-    merges = [flat[at + 4 * i:at + 4 * i + 4] for i in range(plan.n_merge)]
-    rows = flat[at + 4 * plan.n_merge:]
+    merges = [flat[at + 8 * i:at + 8 * i + 5] for i in range(plan.n_merge)]
+    rows = flat[at + 8 * plan.n_merge:]
+    starts = [sum(q_lens[:s]) for s in range(len(q_lens))]
+    for i in range(plan.n_items):
+        s, _, _, _, _, *rest = flat[8 * i:8 * i + 8]
+        assert rest == [starts[s], q_lens[s], lens[s]]
     assert len(rows) == plan.n_rows
     span = lambda s: -(-lens[s] // 64) - (max(0, lens[s] - q_lens[s] - window + 1) // 64 if window else 0)
     assert plan.row_parts == sum(max(1, -(-span(s) // plan.row_per)) for s in rows) if rows else plan.row_parts == 1
     used = sorted(it[4] for it in items if it[4] >= 0)
-    assert used == list(range(plan.slots)) == sorted(m[2] + p for m in merges for p in range(m[3]))
+    assert used == list(range(plan.slots)) == sorted(m[1] + p for m in merges for p in range(m[2]))
     for s, (n, L) in enumerate(zip(q_lens, lens)):
         assert (s in rows) == (0 < n and -(-n * G // 16) <= (1 if d == 256 else 2))
         if s in rows:
@@ -157,9 +161,8 @@ def test_work_lists(heads, hk, d, q_lens, lens, causal, window):
             first, last = L - n + r // G, L - n + (min(r + R, n * G) - 1) // G
             hi = min(L, last + 1) if causal else L
             assert mine[0][2] <= (max(0, first - window + 1) if window else 0) and mine[-1][2] + 64 * mine[-1][3] >= hi
-            assert (len(mine) > 1) == any(m[:2] == [s, r] and m[3] == len(mine) for m in merges)
-    assert sum(1 for it in items) == sum(max(1, sum(m[3] for m in merges if m[:2] == [s, r])) for s, n in enumerate(q_lens) if s not in rows
-                                         for r in range(0, n * G, R))
+            assert (len(mine) > 1) == any(m == [r, mine[0][4], len(mine), starts[s], n] for m in merges)
+    assert len(items) == sum(len([it for it in items if it[0] == s]) for s, n in enumerate(q_lens) if n and s not in rows)
 
 
 def test_room_for_parts():
