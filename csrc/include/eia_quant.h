@@ -27,6 +27,9 @@ struct QuantCache {
   EIA_DEV uint8_t* vscale(int page, int h, int off) const { return vs + page * scales + (long)h * bs + off; }
 };
 
+// A table's entry, held to the pool: what it names outside of it is not read.
+EIA_DEV int quant_page(int page, unsigned top) { return (int)min((unsigned)page, top); }
+
 // 16 bytes that are read once and leave nothing in the caches, or as usual.
 template <bool ONCE> EIA_DEV uint4 quant_load(const void* p) {
   typedef __attribute__((ext_vector_type(4))) unsigned u32x4;

@@ -110,7 +110,7 @@ template <int D> struct Turn {
 
 template <int D, bool NEOX, int TT, int NH, bool ONCE>
 __global__ void __launch_bounds__(256)
-quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float* __restrict__ cos_sin,
+quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float* __restrict__ cos_sin, unsigned last_angle,
                    const int* __restrict__ slots, QuantCache cache, long num_slots, bf16_t* __restrict__ q_out, int T, int Hq,
                    int q_groups) {
   constexpr int TPH = D / 16, HPB = 256 / TPH / TT;        // lanes of a head, heads of a workgroup
@@ -127,7 +127,7 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
     Turn<D> turn;
 #pragma unroll
     for (int n = 0; n < NH; ++n) row[n].ask(src, t, min(h0 + n * HPB, Hq - 1), sub);
-    if (cos_sin) turn.ask(cos_sin + (long)positions[t] * D, sub);
+    if (cos_sin) turn.ask(cos_sin + (long)min((unsigned)positions[t], last_angle) * D, sub);
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       const int h = h0 + n * HPB;
@@ -157,7 +157,7 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
   if (t < T && h < Hkv) {                                  // (whatever the slot: rows are asked for beside it)
     krow.ask(src, t, Hq + h, sub);
     vrow.ask(src, t, Hq + Hkv + h, sub);
-    if (cos_sin) turn.ask(cos_sin + (long)positions[t] * D, sub);
+    if (cos_sin) turn.ask(cos_sin + (long)min((unsigned)positions[t], last_angle) * D, sub);
   }
   if (live) {
     float k[16], v[16];
@@ -296,12 +296,15 @@ quant_read_kernel(QuantCache cache, const int* __restrict__ slots, long num_slot
 
 }  // namespace
 
-// qkv bf16 rows, or part != nullptr: fp32 sums [sk][T][(Hq + 2 Hkv) D].  cos_sin nullptr: no rotation.
+// qkv bf16 rows, or part != nullptr: fp32 sums [sk][T][(Hq + 2 Hkv) D].  cos_sin [angles][D], nullptr: no rotation; positions are held
+// to its rows.
 EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part, int sk, const int* positions, const float* cos_sin,
-                            const int* slots, void* k, void* v, void* ks, void* vs, long codes, long scales, int pages, void* q_out,
+                            int angles, const int* slots, void* k, void* v, void* ks, void* vs, long codes, long scales, int pages, void* q_out,
                             const void* bias, const void* q_norm, const void* k_norm, float eps, int T, int Hq, int Hkv, int D, int bs,
                             int neox, hipStream_t st) {
-  if (T < 0 || Hq <= 0 || Hkv <= 0 || bs <= 0 || bs % QUANT_GROUP || (part && sk < 1) || (!q_norm) != (!k_norm)) return EIA_BAD_SHAPE;
+  if (T < 0 || Hq <= 0 || Hkv <= 0 || bs <= 0 || bs % QUANT_GROUP || (part && sk < 1) || (!q_norm) != (!k_norm) ||
+      (cos_sin && angles < 1))
+    return EIA_BAD_SHAPE;
   if (T == 0) return EIA_OK;
   const QuantSrc src{(const bf16_t*)qkv, part, qkv_stride, (long)T * (Hq + 2 * Hkv) * D, sk, (const bf16_t*)bias, (const bf16_t*)q_norm,
                      (const bf16_t*)k_norm, eps};
@@ -311,7 +314,7 @@ EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part,
     constexpr int hpb = 256 / (D / 16) / TT;                                                                                      \
     const int qg = (Hq + hpb * NH - 1) / (hpb * NH);                                                                              \
     hipLaunchKernelGGL((quant_write_kernel<D, NX, TT, NH, ONCE>), dim3((T + TT - 1) / TT, qg + (Hkv + hpb - 1) / hpb), dim3(256), 0, st, src, \
-                       positions, cos_sin, slots, c, (long)pages * bs, (bf16_t*)q_out, T, Hq, qg);                                \
+                       positions, cos_sin, angles - 1u, slots, c, (long)pages * bs, (bf16_t*)q_out, T, Hq, qg);                                \
   } while (0)
 #define QW_N(D, NX)                                    \
   do {                                                 \

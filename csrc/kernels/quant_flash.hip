@@ -44,6 +44,7 @@ struct Chunk {
   f32x4* po;                         // sums of a part as its lanes hold them [slot][kv head][wave][D / 8][64]
   float2* ml;                        // [slot][kv head][wave][32]
   int groups, longest;               // 16-key groups of a page; tokens that a row of the tables has pages for
+  unsigned top;                      // the last page: tables are held to it
   unsigned magic;
 };
 
@@ -123,7 +124,7 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
   auto fetch = [&] {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int pg = __builtin_amdgcn_readfirstlane(page[i]), id = piece(i);
+      const int pg = quant_page(__builtin_amdgcn_readfirstlane(page[i]), a.top), id = piece(i);
       if (keys_here) {
         const int r = id / (D / 16) % QUANT_GROUP;
         kst[i] = *reinterpret_cast<const uint4*>(cache.key(pg, kvh, off[i] + r, D) + 16 * (id % (D / 16)));
@@ -404,9 +405,10 @@ EIA_API int eia_quant_flash_rows(int D) {
 // items: n of {sequence, first row, first key, key tiles, slot or -1, first query, queries, keys}; merges: n_merge of {first row, first
 // slot, parts, first query, queries, 3 unused}; ws: slots * Hkv * rows of a block * (D + 2) floats.
 EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
-                            const void* vs, long codes, long scales, const int* tables, int bt_stride, int width, const int* items, int n, const int* merges, int n_merge, int slots, float* ws, float scale, int Hq, int Hkv,
+                            const void* vs, long codes, long scales, int pages, const int* tables, int bt_stride, int width,
+                            const int* items, int n, const int* merges, int n_merge, int slots, float* ws, float scale, int Hq, int Hkv,
                             int D, int bs, int causal, int window, int chunk, hipStream_t st) {
-  if (n < 0 || n_merge < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || n > 65535 || n_merge > 65535 ||
+  if (n < 0 || n_merge < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || n > 65535 || n_merge > 65535 || pages < 0 || width < 0 ||
       (slots > 0 && !ws))
     return EIA_BAD_SHAPE;
   if (n == 0) return EIA_OK;
@@ -414,7 +416,7 @@ EIA_API int eia_quant_flash(const void* q, long q_stride, void* out, long out_st
   if (!block) return EIA_UNSUPPORTED;
   const Chunk a{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, bt_stride, Hq, causal, window, chunk,
                 scale * FLASH_LOG2E, reinterpret_cast<f32x4*>(ws), reinterpret_cast<float2*>(ws + (long)slots * Hkv * block * D), groups,
-                (int)std::min<long>((long)width * bs, INT_MAX),
+                pages ? (int)std::min<long>((long)width * bs, INT_MAX) : 0, pages ? pages - 1u : 0u,
                 (unsigned)(((1ull << 32) + groups - 1) / groups)};
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
 #define QF_GO(D)                                                                                                                 \

@@ -34,6 +34,7 @@ struct Rows {
   int2* info;                        // [sequence]: its first part and their number
   int per, least, shift, groups;     // units a part (0: by all units, 2^shift workgroups run at a time, `least` at least); 16-key groups of a page
   int total, longest;                // parts that the launch has room for; tokens that a row of the tables has pages for
+  unsigned top;                      // the last page: tables are held to it
   unsigned magic;                    // 2^32 / groups, rounded up
 };
 
@@ -182,12 +183,12 @@ quant_rows_kernel(Rows r, QuantCache cache) {
   // 64 pages from one on, a lane each: a unit's page is a register's lane and no load in the loop
   auto index_of = [&](int group) { return r.groups == 1 ? group : (int)__umulhi((unsigned)group, r.magic); };
   int held = index_of(min(4 * (ub + w), last));
-  int pages = ub + w < ue ? bt[min(held + lane, index_of(last))] : 0;
+  int pages = ub + w < ue ? quant_page(bt[min(held + lane, index_of(last))], r.top) : 0;
   auto hold = [&](int group) {                              // (the same for the wave)
     const int at = index_of(group);
     if (at < held + 60) return;                             // (a unit lies in four pages at most)
     held = at;
-    pages = bt[min(held + lane, index_of(last))];
+    pages = quant_page(bt[min(held + lane, index_of(last))], r.top);
   };
   auto off_of = [&](int group) { return QUANT_GROUP * (group - index_of(group) * r.groups); };
   // Where a unit's keys and values lie: page and first token in it, one pair for a unit that one page holds (UNI), else a
@@ -390,7 +391,8 @@ quant_rows_merge_kernel(Rows r, int Hkv) {
   __shared__ f32x4 so[PG][LANES];
   const int kvh = blockIdx.x, G = r.Hq / Hkv, col = blockIdx.z, pg = threadIdx.x / LANES, d = threadIdx.x % LANES;
   const int s = r.list ? r.list[blockIdx.y] : blockIdx.y;
-  const int2 at = r.info[s];
+  const int2 at = r.info[s];                                // (of a sequence whose parts had no room in the launch: anything)
+  if (at.x < 0 || at.x >= r.total) return;
   const int q0 = r.cu ? r.cu[s] : s, qlen = r.cu ? r.cu[s + 1] - q0 : 1, parts = min(at.y, r.total - at.x);
   if (parts <= 1 || col >= qlen * G) return;
   const long base = ((long)at.x * Hkv + kvh) * (16 * NC) + col, step = (long)Hkv * (16 * NC);
@@ -447,10 +449,10 @@ quant_rows_merge_kernel(Rows r, int Hkv) {
 // head of a kv head); per: units of 64 keys a part (0: all over 2^shift workgroups, `least` at least); parts: that many at most, n alone if no sequence
 // is cut; ws (parts > n): parts * Hkv * 16 * tiles * (D + 2) floats, then 2 ints for every sequence.
 EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
-                           const void* vs, long codes, long scales, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
+                           const void* vs, long codes, long scales, int pages, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
                            const int* list, int n, float scale, int Hq, int Hkv, int D, int bs, int causal, int window, int chunk,
                            int tiles, int parts, int per, int least, int shift, float* ws, hipStream_t st) {
-  if (n < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || parts < n || width < 0 || (parts > n && !ws) || parts > 65535 ||
+  if (n < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || parts < n || pages < 0 || width < 0 || (parts > n && !ws) || parts > 65535 ||
       per < 0 || least < 1 || shift < 0 || shift > 24 || tiles < 1)
     return EIA_BAD_SHAPE;
   if (n == 0) return EIA_OK;
@@ -458,7 +460,8 @@ EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_str
   const long rows = (long)parts * Hkv * 16 * tiles;
   Rows r{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, list, bt_stride, n, Hq, causal, window, chunk,
          scale * FLASH_LOG2E, nullptr, nullptr, nullptr, per, least, shift, groups, parts,
-         (int)std::min<long>((long)width * bs, INT_MAX), (unsigned)(((1ull << 32) + groups - 1) / groups)};
+         pages ? (int)std::min<long>((long)width * bs, INT_MAX) : 0, pages ? pages - 1u : 0u,
+         (unsigned)(((1ull << 32) + groups - 1) / groups)};
   if (parts > n) {
     r.po = reinterpret_cast<f32x4*>(ws);
     r.ml = reinterpret_cast<float2*>(ws + rows * D);

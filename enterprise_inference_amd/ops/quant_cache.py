@@ -187,7 +187,8 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
     """qkv [T, (Hq + 2 Hkv) D] -> q [T, Hq, D]; keys and values go into the 8-bit cache (``rope_qkv_cache`` for it).
 
     ``qkv`` may be a ``gemm.SplitK``, summed here.  Bias, per-head norms and rotation are fp32, rounded once: queries to bf16,
-    keys and values to their codes.  Slots are distinct; tokens whose slot is outside the cache write nothing."""
+    keys and values to their codes.  Slots are distinct; tokens whose slot is outside the cache write nothing.  Positions lie in the
+    rotary table."""
     part = None
     if not isinstance(qkv, torch.Tensor):
         from .gemm import SplitK
@@ -212,7 +213,7 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
         table, neox = rotary.cos_sin, rotary.is_neox
         if not (positions is not None and positions.dtype is torch.int32 and positions.numel() >= T and positions.stride(-1) == 1):
             raise ValueError("rope_qkv_quant: positions int32[T]")
-        if not (table.shape[1] == head_dim and table.dtype is torch.float32 and table.is_contiguous()):
+        if not (table.shape[0] > 0 and table.shape[1] == head_dim and table.dtype is torch.float32 and table.is_contiguous()):
             raise ValueError("rope_qkv_quant: cos | sin fp32 [positions, D]")
     src = part.part if part is not None else qkv
     if part is None and not (cache._hip and qkv.is_cuda and qkv.dtype is torch.bfloat16):
@@ -232,7 +233,7 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
     q = torch.empty((T, num_heads, head_dim), dtype=torch.bfloat16, device=device)
     _launch("rope_qkv_quant", lib().eia_quant_write, device, None if part is not None else ptr(qkv),
             0 if part is not None else qkv.stride(0), ptr(src) if part is not None else None, part.sk if part is not None else 0,
-            ptr(positions), ptr(table), ptr(slot_mapping), *cache._args, cache.pages, ptr(q), ptr(bias), ptr(q_norm_w), ptr(k_norm_w),
+            ptr(positions), ptr(table), 0 if table is None else table.shape[0], ptr(slot_mapping), *cache._args, cache.pages, ptr(q), ptr(bias), ptr(q_norm_w), ptr(k_norm_w),
             float(norm_eps), T, num_heads, num_kv_heads, head_dim, cache.block_size, 1 if neox else 0)
     return q
 
@@ -252,7 +253,7 @@ def quant_read(cache: QuantKVCache, slots: torch.Tensor, dtype: torch.dtype = to
 
 
 # ------------------------------------------------------------------------------ attention
-def _check_attention(name, q, cache, block_tables, seq_lens, n, scale, out):
+def _check_attention(name, q, cache, block_tables, seq_lens, n, scale, window, chunk, out):
     """(whether the kernels take it, tokens, heads); ``n`` sequences."""
     T, Hq, D = q.shape
     if not (D == cache.head_dim and Hq % cache.num_kv_heads == 0):
@@ -263,6 +264,8 @@ def _check_attention(name, q, cache, block_tables, seq_lens, n, scale, out):
         raise ValueError(f"{name}: metadata rows < sequences")
     if not scale > 0.0:
         raise ValueError(f"{name}: scale > 0")
+    if (window or 0) < 0 or (chunk or 0) < 0:
+        raise ValueError(f"{name}: window, chunk size >= 0")
     if out is not None and not (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device):
         raise ValueError(f"{name}: out like q")
     if not (cache._hip and q.is_cuda and q.dtype is torch.bfloat16):
@@ -295,7 +298,7 @@ def _launch_rows(name, q, out, cache, block_tables, seq_lens, cu, seqs, n, seque
     ws = torch.empty(parts * cache.num_kv_heads * 16 * tiles * (D + 2) + 2 * sequences, dtype=torch.float32,
                      device=cache.device) if parts > n else None
     _launch(name, lib().eia_quant_rows, cache.device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *cache._args,
-            block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu, seqs, n, float(scale), Hq,
+            cache.pages, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu, seqs, n, float(scale), Hq,
             cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, ROW_SHIFT,
             ptr(ws))
 
@@ -320,7 +323,7 @@ def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tenso
     Rows of length 0 become zeros.  Nothing is read back: lengths and tables may change under a captured graph, up to the
     tables' width."""
     B = q.shape[0]
-    hip, _, Hq = _check_attention("quant_decode", q, cache, block_tables, seq_lens, B, scale, out)
+    hip, _, Hq = _check_attention("quant_decode", q, cache, block_tables, seq_lens, B, scale, sliding_window, chunk_size, out)
     if not hip:
         rows = [_attend_plain(q[b:b + 1], cache, block_tables[b], int(seq_lens[b]), scale, True, sliding_window, chunk_size) for b in range(B)]
         r = torch.cat(rows).to(q.dtype) if B else q.clone()
@@ -361,6 +364,8 @@ class QuantPrefillPlan:
     row_parts: int = 1
     row_per: int = 0
 
+    stream = ready = None                  # of the lists' upload
+
     def __post_init__(self):
         self.tokens, self.longest = sum(self.q_lens), max(self.kv_lens, default=0)
 
@@ -378,10 +383,15 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
     """Work lists of ``quant_prefill`` for chunks of ``q_lens`` new tokens that end at ``kv_lens`` cached ones.
 
     Sequences of few (query, head) rows go to the kernel that streams the cache for one block of them; the others are cut into
-    blocks of rows, the long ones along the keys too where else the launch would wait for them."""
+    blocks of rows, the long ones along the keys too where else the launch would wait for them.  The lists are uploaded behind the
+    current stream's work; a program that replays a captured ``quant_prefill`` keeps the plan."""
     q_lens, kv_lens = [int(n) for n in q_lens], [int(n) for n in kv_lens]
     require(len(q_lens) == len(kv_lens) and all(n >= 0 for n in q_lens + kv_lens), "quant_prefill_plan: lengths")
     require(num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim in HEAD_DIMS, "quant_prefill_plan: heads")
+    require((sliding_window or 0) >= 0 and (chunk_size or 0) >= 0, "quant_prefill_plan: window, chunk size >= 0")
+    device = torch.device(device)
+    # (a replay would read host memory that is another's by then)
+    require(not (device.type == "cuda" and torch.cuda.is_current_stream_capturing()), "quant_prefill_plan: before a graph is captured")
     plan = QuantPrefillPlan(q_lens, kv_lens, num_heads, num_kv_heads, head_dim, causal, sliding_window, chunk_size, None)
     G = num_heads // num_kv_heads
     few, blocks, first = [], [], [0, *itertools.accumulate(q_lens)]
@@ -423,7 +433,11 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
         items.sort(key=lambda b: -b[0])
         plan.n_items, plan.n_merge = len(items), len(merges) // 8
     flat = [x for _, it in items for x in it] + merges + few
-    plan.lists = torch.tensor(flat, dtype=torch.int32, pin_memory=torch.device(device).type == "cuda").to(device, non_blocking=True)
+    plan.lists = torch.tensor(flat, dtype=torch.int32, pin_memory=device.type == "cuda").to(device, non_blocking=True)
+    if device.type == "cuda":                     # (a copy behind the stream's work: other streams wait for it)
+        plan.stream = torch.cuda.current_stream(plan.lists.device)
+        plan.ready = torch.cuda.Event()
+        plan.ready.record(plan.stream)
     return plan
 
 
@@ -476,7 +490,7 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
     cache already holds -> out [T, Hq, D] (``paged_prefill`` for the 8-bit cache).  ``plan`` holds the lengths that ``cu_q`` and
     ``seq_lens`` hold on the device; rows that see no key become zeros."""
     n = len(plan.q_lens)
-    hip, T, Hq = _check_attention("quant_prefill", q, cache, block_tables, seq_lens, n, scale, out)
+    hip, T, Hq = _check_attention("quant_prefill", q, cache, block_tables, seq_lens, n, scale, plan.sliding_window, plan.chunk_size, out)
     D = cache.head_dim
     if not (plan.num_heads == Hq and plan.num_kv_heads == cache.num_kv_heads and plan.head_dim == D):
         raise ValueError("quant_prefill: plan of other heads")
@@ -493,13 +507,18 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
         return r if out is None else out.copy_(r)
     if not (plan.lists.device == cu_q.device == cache.device):
         raise ValueError("quant_prefill: plan and chunks on the cache's device")
+    if plan.stream.cuda_stream != torch._C._cuda_getCurrentRawStream(cache.device.index) and not torch.cuda.is_current_stream_capturing():
+        here = torch.cuda.current_stream(cache.device)
+        here.wait_event(plan.ready)
+        plan.lists.record_stream(here)
     o = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=cache.device) if out is None else out
     base, window, chunk = plan.lists.data_ptr(), plan.sliding_window or 0, plan.chunk_size or 0
     if plan.n_items:
         ws = torch.empty(plan.slots * cache.num_kv_heads * FLASH_ROWS[D] * (D + 2), dtype=torch.float32, device=cache.device) if plan.slots else None
         _launch("quant_prefill", lib().eia_quant_flash, cache.device, q.data_ptr(), q.stride(0), o.data_ptr(), o.stride(0), *cache._args,
-                block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], base, plan.n_items, base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq, cache.num_kv_heads, D,
-                cache.block_size, 1 if plan.causal else 0, window, chunk)
+                cache.pages, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], base, plan.n_items,
+                base + 32 * plan.n_items, plan.n_merge, plan.slots, ptr(ws), float(scale), Hq, cache.num_kv_heads, D, cache.block_size,
+                1 if plan.causal else 0, window, chunk)
     if plan.n_rows:
         _launch_rows("quant_prefill", q, o, cache, block_tables, seq_lens, cu_q.data_ptr(), base + 32 * (plan.n_items + plan.n_merge),
                      plan.n_rows, n, scale, plan.causal, window, chunk, plan.row_tiles, plan.row_parts, plan.row_per)

@@ -231,3 +231,8 @@ def test_what_is_refused():
         Q.quant_prefill(q, c, bt, lens, cu, Q.quant_prefill_plan([1, 2], [5, 40], 4, 2, 64, "cpu"), 0.1)
     with pytest.raises(ValueError):
         Q.quant_prefill_plan([1], [5, 6], 4, 2, 64, "cpu")
+    for kw in (dict(sliding_window=-1), dict(chunk_size=-8)):
+        with pytest.raises(ValueError):
+            Q.quant_decode(q, c, bt, lens, 0.1, **kw)
+        with pytest.raises(ValueError):
+            Q.quant_prefill_plan([1], [5], 4, 2, 64, "cpu", **kw)

@@ -198,7 +198,7 @@ def test_decode_long(H, hk, D, bs):
 
 @pytest.mark.parametrize("H,hk,D,bs", [(8, 2, 128, 128), (4, 4, 64, 16), (6, 2, 256, 48), (7, 1, 128, 64), (5, 1, 64, 32), (32, 1, 128, 16)])
 @pytest.mark.parametrize("q_lens,lens", [([3], [3]), ([5, 2], [200, 70]), ([65], [65]), ([33, 1, 0, 90], [100, 5, 9, 90]), ([70], [400])])
-@pytest.mark.parametrize("causal,window,chunk", [(True, 0, 0), (True, 20, 0), (True, 0, 32), (False, 0, 0)])
+@pytest.mark.parametrize("causal,window,chunk", [(True, 0, 0), (True, 20, 0), (True, 0, 32), (False, 0, 0), (False, 20, 0)])
 def test_chunks(H, hk, D, bs, q_lens, lens, causal, window, chunk):
     _attend(H, hk, D, bs, q_lens, lens, causal, window, chunk)
 
@@ -363,3 +363,218 @@ def test_large_writes_and_reads():
     whole, half = Q.quant_read(a, slots), [Q.quant_read(a, slots[:8000]), Q.quant_read(a, slots[8000:])]
     for i in range(2):
         assert torch.equal(whole[i], torch.cat([h[i] for h in half]))
+
+
+def _dense64(q, parts, bt_row, L, n, causal=True, scale=0.02):
+    """float64 on the GPU for one sequence's n last tokens: (out, weighted magnitudes) [n, H, D]."""
+    H, hk = q.shape[1], parts[0].shape[1]
+    out, mag = [], []
+    for h in range(H):
+        k, v = (x.cuda() for x in C.row64(parts, bt_row, L, h * hk // H))
+        s = q[:, h].double() @ k.T * scale
+        if causal:
+            s = s.masked_fill(torch.arange(L, device="cuda")[None] > torch.arange(L - n, L, device="cuda")[:, None], -math.inf)
+        w = torch.softmax(s, -1)
+        out.append(w @ v), mag.append(w @ v.abs())
+    return torch.stack(out, 1).cpu(), torch.stack(mag, 1).cpu()
+
+
+@pytest.mark.parametrize("bs", [16, 48, 128])
+def test_decode_parts_of_many_pages(bs):
+    """Enough rows that a part is longer than 64 small pages."""
+    Q = _q()
+    g = torch.Generator().manual_seed(bs)
+    lens = [4000 - 37 * i for i in range(40)]
+    bt, pages = C.tables(g, lens, bs)
+    parts = C.raw_cache(g, pages, 8, bs, 64)
+    C.spoil_behind(parts, bt, lens, bs)
+    q = torch.randn(40, 16, 64, generator=g).to(BF).cuda()
+    got = Q.quant_decode(q, _on_gpu(parts), bt.cuda(), _i32(lens), 0.02)
+    for s in (0, 17, 39):
+        C.check_attention(got[s:s + 1].cpu(), *_dense64(q[s:s + 1], parts, bt[s], lens[s], 1))
+
+
+@pytest.mark.parametrize("D,H,hk", [(128, 8, 2), (64, 4, 4), (256, 4, 2)])
+def test_long_chunks(D, H, hk):
+    """Several rounds of blocks; more than one block of rows behind a long context."""
+    Q = _q()
+    g = torch.Generator().manual_seed(D)
+    q_lens, lens = [700, 9, 333], [5200, 3000, 333]
+    bt, pages = C.tables(g, lens, 32)
+    parts = C.raw_cache(g, pages, hk, 32, D)
+    C.spoil_behind(parts, bt, lens, 32)
+    q = torch.randn(sum(q_lens), H, D, generator=g).to(BF).cuda()
+    plan = Q.quant_prefill_plan(q_lens, lens, H, hk, D, "cuda")
+    got = Q.quant_prefill(q, _on_gpu(parts), bt.cuda(), _i32(lens), _i32([0, 700, 709, 1042]), plan, 0.02)
+    at = 0
+    for s, (n, L) in enumerate(zip(q_lens, lens)):
+        C.check_attention(got[at:at + n].cpu(), *_dense64(q[at:at + n], parts, bt[s], L, n))
+        at += n
+
+
+def test_pools_past_32_bits():
+    """More than 4 GiB of keys, and of values: the last pages."""
+    Q = _q()
+    H, hk, D, bs, pages, n = 8, 8, 128, 128, 33000, 300
+    cache = Q.QuantKVCache.allocate(pages, hk, bs, D, "cuda")
+    assert cache.k.stride(0) * (pages - 3) > 1 << 32
+    bt = _i32([[pages - 1, pages - 3, pages - 2], [0, 1, 2]])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.randn(2 * n, (H + 2 * hk) * D, generator=g, device="cuda").to(BF)
+    t = torch.arange(n, device="cuda")
+    slots = torch.cat([(bt[s][t // bs] * bs + t % bs) for s in range(2)]).to(torch.int32)
+    q = Q.rope_qkv_quant(qkv, None, None, slots, cache, H, hk, D)
+    # the same tokens in a small pool
+    small = Q.QuantKVCache.allocate(6, hk, bs, D, "cuda")
+    st = _i32([[0, 1, 2], [3, 4, 5]])
+    ss = torch.cat([(st[s][t // bs] * bs + t % bs) for s in range(2)]).to(torch.int32)
+    Q.rope_qkv_quant(qkv, None, None, ss, small, H, hk, D)
+    for a, b in zip(Q.quant_read(cache, slots), Q.quant_read(small, ss)):
+        assert torch.equal(a, b)
+    lens, cu = _i32([n, n]), _i32([0, n, 2 * n])
+    plan = Q.quant_prefill_plan([n, n], [n, n], H, hk, D, "cuda")
+    assert torch.equal(Q.quant_prefill(q, cache, bt, lens, cu, plan, 0.1), Q.quant_prefill(q, small, st, lens, cu, plan, 0.1))
+    last = q[[n - 1, 2 * n - 1]].contiguous()
+    assert torch.equal(Q.quant_decode(last, cache, bt, lens, 0.1), Q.quant_decode(last, small, st, lens, 0.1))
+
+
+def test_a_captured_step_replays():
+    """Write, chunk and decode in one graph, replayed with other inputs and eager work between."""
+    Q = _q()
+    from enterprise_inference_amd.ops.rotary import RotaryCache
+    H, hk, D, bs = 8, 2, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rot = RotaryCache(D, 2000, 10000.0, None, torch.device("cuda"))
+    q_lens, lens, B = [150, 3], [1500, 700], 2
+    bt = torch.randperm(60, generator=g, device="cuda")[:50].view(2, 25).to(torch.int32)
+    dbt = torch.randperm(60, generator=g, device="cuda")[:30].view(2, 15).to(torch.int32)
+    cache = Q.QuantKVCache.allocate(60, hk, bs, D, "cuda")
+    fill = torch.randint(0, 100, cache.k.shape, generator=g, device="cuda").to(torch.uint8)
+    cache.k.view(torch.uint8).copy_(fill), cache.v.view(torch.uint8).copy_(fill.view(cache.v.shape))
+    cache.k_scale.fill_(124), cache.v_scale.fill_(125)
+    T = B + sum(q_lens)
+    qkv = torch.randn(T, (H + 2 * hk) * D, generator=g, device="cuda").to(BF)
+    pos, slots = torch.randint(0, 2000, (T,), generator=g, device="cuda").to(torch.int32), torch.randperm(60 * bs, generator=g, device="cuda")[:T].to(torch.int32)
+    dlens, plens, cu = _i32([900, 33]), _i32(lens), _i32([0, 150, 153])
+    plan = Q.quant_prefill_plan(q_lens, lens, H, hk, D, "cuda")
+
+    def step():
+        q = Q.rope_qkv_quant(qkv, pos, rot, slots, cache, H, hk, D)
+        return torch.cat([Q.quant_decode(q[:B], cache, dbt, dlens, 0.05), Q.quant_prefill(q[B:], cache, bt, plens, cu, plan, 0.05)])
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(4):
+        qkv.copy_(torch.randn(qkv.shape, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, step()) and bool(torch.isfinite(got).all())
+
+
+def test_two_streams_at_once():
+    Q = _q()
+    g = torch.Generator().manual_seed(13)
+    lens = [3000, 2500, 1]
+    bt, pages = C.tables(g, lens, 64)
+    parts = C.raw_cache(g, pages, 2, 64, 128)
+    cache, dbt, dl = _on_gpu(parts), bt.cuda(), _i32(lens)
+    qs = [torch.randn(3, 8, 128, generator=g).to(BF).cuda() for _ in range(2)]
+    chunk = torch.randn(90, 8, 128, generator=g).to(BF).cuda()
+    args = (chunk, cache, dbt[:1], dl[:1], _i32([0, 90]))
+    first = [Q.quant_decode(q, cache, dbt, dl, 0.02) for q in qs]
+    plan = Q.quant_prefill_plan([90], [3000], 8, 2, 128, "cuda")
+    whole = Q.quant_prefill(*args, plan, 0.02)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(Q.quant_decode(qs[i], cache, dbt, dl, 0.02))
+    other = Q.quant_prefill_plan([90], [3000], 8, 2, 128, "cuda")              # made on this stream, used on another
+    with torch.cuda.stream(streams[0]):
+        late = Q.quant_prefill(*args, other, 0.02)
+    torch.cuda.synchronize()
+    assert torch.equal(late, whole)
+    for i in range(2):
+        assert all(torch.equal(x, first[i]) for x in got[i])
+
+
+def test_a_query_that_is_no_number_stays_alone():
+    Q = _q()
+    g = torch.Generator().manual_seed(17)
+    for q_lens, lens, hk in (([1, 1], [70, 300], 1), ([5], [300], 1), ([90], [300], 2)):
+        bt, pages = C.tables(g, lens, 64)
+        parts = C.raw_cache(g, pages, hk, 64, 128)
+        q = torch.randn(sum(q_lens), 4, 128, generator=g).to(BF)
+        bad = q.clone()
+        bad[1, 2, 5] = math.nan
+        plan = Q.quant_prefill_plan(q_lens, lens, 4, hk, 128, "cuda")
+        cu = _i32([0] + q_lens).cumsum(0).to(torch.int32)
+        a, b = (Q.quant_prefill(x.cuda(), _on_gpu(parts), bt.cuda(), _i32(lens), cu, plan, 0.02) for x in (q, bad))
+        assert bool(torch.isnan(b[1, 2]).all())
+        b[1, 2] = a[1, 2]
+        assert torch.equal(a, b)
+
+
+def test_entries_outside_the_pool_and_positions_outside_the_table():
+    """Held to the last page, to the last row and to the table's width: nothing outside is read."""
+    Q = _q()
+    from enterprise_inference_amd.ops.rotary import RotaryCache
+    g = torch.Generator().manual_seed(21)
+    for bs in (48, 64):
+        cache = _on_gpu(C.raw_cache(g, 5, 2, bs, 128))
+        q = torch.randn(3, 8, 128, generator=g).to(BF).cuda()
+        bad, held = _i32([[0, -1, 2], [1 << 30, 3, 1], [5, 0, 0]]), _i32([[0, 4, 2], [4, 3, 1], [4, 0, 0]])
+        lens, long = _i32([3 * bs, 2 * bs + 1, 7]), _i32([1 << 30, 2 * bs + 1, 7])
+        want = Q.quant_decode(q, cache, held, lens, 0.02)
+        for bt in (bad, held):
+            for n in (lens, long):
+                assert torch.equal(Q.quant_decode(q, cache, bt, n, 0.02), want)
+        chunk, cu = torch.randn(100, 8, 128, generator=g).to(BF).cuda(), _i32([0, 2, 100])
+        plan = Q.quant_prefill_plan([2, 98], [3 * bs, 2 * bs + 1], 8, 2, 128, "cuda")
+        assert torch.equal(*(Q.quant_prefill(chunk, cache, bt, lens, cu, plan, 0.02) for bt in (bad, held)))
+    rot = RotaryCache(128, 50, 10000.0, None, torch.device("cuda"))
+    qkv, slots = torch.randn(3, 12 * 128, generator=g).to(BF).cuda(), _i32([1, 2, 3])
+    a, b = (Q.rope_qkv_quant(qkv, _i32(p), rot, slots, cache, 8, 2, 128) for p in ([49, 49, 7], [-1, 1 << 30, 7]))
+    assert torch.equal(a, b)
+
+
+def test_no_pages_and_no_width():
+    Q = _q()
+    q, cu = torch.ones(2, 4, 64, dtype=BF, device="cuda"), _i32([0, 2])
+    for pages, width in ((0, 1), (1, 0)):
+        cache = Q.QuantKVCache.allocate(pages, 2, 16, 64, "cuda")
+        bt = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+        assert not Q.quant_decode(q, cache, bt, _i32([0, 0]), 0.1).any()
+        assert not Q.quant_decode(q, cache, bt, _i32([9, 9]), 0.1).any()
+        assert not Q.quant_prefill(q, cache, bt, _i32([0]), cu, Q.quant_prefill_plan([2], [0], 4, 2, 64, "cuda"), 0.1).any()
+
+
+def test_a_plan_is_made_before_the_capture():
+    Q = _q()
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(ValueError):
+            Q.quant_prefill_plan([90], [3000], 8, 2, 128, "cuda")
+    graph.replay()
+    assert x.sum().item() == 4
+
+
+def test_more_decode_rows_than_lanes():
+    """The sequences' lengths are found 64 at a time."""
+    Q = _q()
+    g = torch.Generator().manual_seed(130)
+    lens = [int(x) for x in torch.randint(0, 700, (130,), generator=g)]
+    lens[64], lens[65], lens[129] = 0, 699, 1
+    bt, pages = C.tables(g, lens, 64)
+    parts = C.raw_cache(g, pages, 2, 64, 128)
+    q = torch.randn(130, 8, 128, generator=g).to(BF)
+    got = Q.quant_decode(q.cuda(), _on_gpu(parts), bt.cuda(), _i32(lens), 0.02)
+    C.check_attention(got.cpu(), *C.attend64(q, parts, bt, [1] * 130, lens, 0.02))
