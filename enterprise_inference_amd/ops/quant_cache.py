@@ -11,6 +11,7 @@ Step layout, block tables, slots and lengths are those of ``ops.attention`` and 
 from __future__ import annotations
 
 import dataclasses
+import functools
 import heapq
 import itertools
 from typing import List, Optional, Sequence, Tuple
@@ -171,6 +172,14 @@ def _attend_plain(q, cache, table, L, scale, causal, window, chunk):
 
 
 # ------------------------------------------------------------------------------ write and read
+# Calls of few tokens are bound by the host: a launch takes it 3 us, torch.empty 1.65 (empty_strided 1.26, empty_like 1.15), a tensor's
+# attribute 0.05 to 0.1.
+def _empty(shape, device) -> torch.Tensor:
+    """bf16 [n, heads, D]."""
+    d = shape[2]
+    return torch.empty_strided(shape, (shape[1] * d, d, 1), dtype=torch.bfloat16, device=device)
+
+
 def _launch(name: str, call, device: torch.device, *args) -> None:
     """``call`` on the device's current stream.  A launch belongs to the device that is current: the tensors' one."""
     index = device.index
@@ -230,7 +239,7 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
     if not all(t is None or t.device == device for t in (cache, slot_mapping, positions if table is not None else None, table, bias, q_norm_w,
                                                          k_norm_w)):
         raise ValueError("rope_qkv_quant: one device")
-    q = torch.empty((T, num_heads, head_dim), dtype=torch.bfloat16, device=device)
+    q = _empty((T, num_heads, head_dim), device)
     _launch("rope_qkv_quant", lib().eia_quant_write, device, None if part is not None else ptr(qkv),
             0 if part is not None else qkv.stride(0), ptr(src) if part is not None else None, part.sk if part is not None else 0,
             ptr(positions), ptr(table), 0 if table is None else table.shape[0], ptr(slot_mapping), *cache._args, cache.pages, ptr(q), ptr(bias), ptr(q_norm_w), ptr(k_norm_w),
@@ -245,9 +254,10 @@ def quant_read(cache: QuantKVCache, slots: torch.Tensor, dtype: torch.dtype = to
     if not (cache._hip and dtype is torch.bfloat16):
         return tuple(t.to(dtype) for t in _read_rows(cache, slots))
     shape = (slots.shape[0], cache.num_kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=cache.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.device)
-    _launch("quant_read", lib().eia_quant_read, cache.device, *cache._args, cache.pages, slots.data_ptr(), shape[0], k.data_ptr(),
+    device = cache.device
+    k = _empty(shape, device)
+    v = torch.empty_like(k)
+    _launch("quant_read", lib().eia_quant_read, device, *cache._args, cache.pages, slots.data_ptr(), shape[0], k.data_ptr(),
             v.data_ptr(), shape[1], shape[2], cache.block_size)
     return k, v
 
@@ -270,12 +280,12 @@ def _check_attention(name, q, cache, block_tables, seq_lens, n, scale, window, c
         raise ValueError(f"{name}: out like q")
     if not (cache._hip and q.is_cuda and q.dtype is torch.bfloat16):
         return False, T, Hq
-    for t in (q, out):
-        if t is not None:
-            s = t.stride()
-            if not (s[2] == 1 and s[1] == D and s[0] % 8 == 0 and t.data_ptr() % 16 == 0):
-                raise ValueError(f"{name}: rows of q and out on 16 bytes")
-    if not (q.device == cache.device == block_tables.device == seq_lens.device):
+    for t in (q, out) if out is not None else (q,):
+        s = t.stride()
+        if not (s[2] == 1 and s[1] == D and s[0] % 8 == 0 and t.data_ptr() % 16 == 0):
+            raise ValueError(f"{name}: rows of q and out on 16 bytes")
+    device = cache.device
+    if not (q.device == device and block_tables.device == device and seq_lens.device == device):
         raise ValueError(f"{name}: one device")
     if not (block_tables.stride(1) == 1 and seq_lens.stride(-1) == 1):
         raise ValueError(f"{name}: contiguous metadata")
@@ -294,10 +304,10 @@ ROW_LONG = 48                 # longer parts are halved
 
 
 def _launch_rows(name, q, out, cache, block_tables, seq_lens, cu, seqs, n, sequences, scale, causal, window, chunk, tiles, parts, per):
-    _, Hq, D = q.shape
-    ws = torch.empty(parts * cache.num_kv_heads * 16 * tiles * (D + 2) + 2 * sequences, dtype=torch.float32,
-                     device=cache.device) if parts > n else None
-    _launch(name, lib().eia_quant_rows, cache.device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *cache._args,
+    Hq, D, device = q.shape[1], cache.head_dim, cache.device
+    ws = torch.empty_strided((parts * cache.num_kv_heads * 16 * tiles * (D + 2) + 2 * sequences,), (1,), dtype=torch.float32,
+                             device=device) if parts > n else None
+    _launch(name, lib().eia_quant_rows, device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *cache._args,
             cache.pages, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu, seqs, n, float(scale), Hq,
             cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, ROW_SHIFT,
             ptr(ws))
@@ -316,6 +326,16 @@ def _row_parts(n: int, units: int, num_kv_heads: int) -> int:
     return min(n * max(1, -(-units // ROW_LEAST)), (rounds << ROW_SHIFT) // num_kv_heads + n)
 
 
+@functools.lru_cache(maxsize=256)
+def _decode_grid(B: int, span: int, group: int, num_kv_heads: int, head_dim: int, window, chunk) -> Tuple[int, int]:
+    """(row tiles, room for parts) of B rows of at most ``span`` tokens."""
+    units = -(-span // UNIT)
+    for w in (window, chunk):
+        if w:
+            units = min(units, -(-w // UNIT) + 1)
+    return _row_tiles(group, head_dim), _row_parts(B, units, num_kv_heads)
+
+
 def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
                  sliding_window: Optional[int] = None, chunk_size: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [B, Hq, D], one token a sequence, the last of ``seq_lens`` [B] -> out [B, Hq, D] (``paged_decode`` for the 8-bit cache).
@@ -328,18 +348,13 @@ def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tenso
         rows = [_attend_plain(q[b:b + 1], cache, block_tables[b], int(seq_lens[b]), scale, True, sliding_window, chunk_size) for b in range(B)]
         r = torch.cat(rows).to(q.dtype) if B else q.clone()
         return r if out is None else out.copy_(r)
-    o = torch.empty((B, Hq, cache.head_dim), dtype=torch.bfloat16, device=cache.device) if out is None else out
-    tiles = _row_tiles(Hq // cache.num_kv_heads, cache.head_dim)
+    tiles, parts = _decode_grid(B, block_tables.shape[1] * cache.block_size, Hq // cache.num_kv_heads, cache.num_kv_heads, cache.head_dim,
+                                sliding_window, chunk_size)
     if tiles == 0:
         raise ValueError("quant_decode: too many query heads a kv head")
+    o = _empty((B, Hq, cache.head_dim), cache.device) if out is None else out
     if B == 0:
         return o
-    span = block_tables.shape[1] * cache.block_size
-    units = -(-span // UNIT)
-    for w in (sliding_window, chunk_size):
-        if w:
-            units = min(units, -(-w // UNIT) + 1)
-    parts = _row_parts(B, units, cache.num_kv_heads)
     _launch_rows("quant_decode", q, o, cache, block_tables, seq_lens, None, None, B, B, scale, True, sliding_window, chunk_size, tiles, parts, 0)
     return o
 
@@ -511,7 +526,7 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
         here = torch.cuda.current_stream(cache.device)
         here.wait_event(plan.ready)
         plan.lists.record_stream(here)
-    o = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=cache.device) if out is None else out
+    o = _empty((T, Hq, D), cache.device) if out is None else out
     base, window, chunk = plan.lists.data_ptr(), plan.sliding_window or 0, plan.chunk_size or 0
     if plan.n_items:
         ws = torch.empty(plan.slots * cache.num_kv_heads * FLASH_ROWS[D] * (D + 2), dtype=torch.float32, device=cache.device) if plan.slots else None
