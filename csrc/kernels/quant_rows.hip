@@ -32,7 +32,7 @@ struct Rows {
   f32x4* po;                         // sums [part][kv head][column][D / 4]
   float2* ml;                        // maxima (log2), sums of weights [part][kv head][column]
   int2* info;                        // [sequence]: its first part and their number
-  int per, least, shift, groups;     // units a part (0: by all units, 2^shift workgroups run at a time, `least` at least); 16-key groups of a page
+  int per, least, share, groups;     // units a part (0: all over `share` workgroups, `least` at least); 16-key groups of a page
   int total, longest;                // parts that the launch has room for; tokens that a row of the tables has pages for
   unsigned top;                      // the last page: tables are held to it
   unsigned magic;                    // 2^32 / groups, rounded up
@@ -64,11 +64,10 @@ EIA_DEV Span rows_span(const Rows& r, int L, int qlen) {
 }
 
 // Units a part for so many in all: one round of the workgroups that run at a time, or two where that leaves parts of more than
-// RLONG (their ends are apart then).  32 heads on 8, us at 2^8, 2^9, 2^10, 2^11 parts: 65 rows of 1000 to 2000 keys 48.2, 43.9, 45.2,
-// 46.7; 64 of 2048 47.5, 47.4, 50.0, 53.1; 32 of 8192 to 16384 192, 152, 144, 142; 8 of 1000 to 2000 15.5, 12.2, 12.0, 12.2.
+// RLONG (their ends are apart then: 32 heads on 8, 32 rows of 8192 to 16384 keys in 512 parts 152 us, in 1024 144).
 constexpr int RLONG = 48;
 EIA_DEV int rows_per(const Rows& r, long units) {
-  const int one = (int)((units + (1 << r.shift) - 1) >> r.shift), two = (one + 1) / 2;
+  const int one = (int)((units + r.share - 1) / r.share), two = (one + 1) / 2;
   return max(r.least, min(one, max(two, RLONG)));
 }
 
@@ -136,7 +135,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
   constexpr bool AHEAD = D <= 128;   // keys are asked for a unit ahead; 256 channels: that costs the second workgroup on a CU
   __shared__ bool there;
   __shared__ float sm[RW][16 * NC], sl[RW][16 * NC];
-  __shared__ __align__(16) float so[RW][D][16 * NC + 1];
+  __shared__ __align__(16) float so[RW][16 * NC][D + 4];      // (rows 16 bytes apart from a power of two)
   const int kvh = blockIdx.x, Hkv = cache.Hkv, G = r.Hq / Hkv;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const Part at = rows_part(r, Hkv, blockIdx.y);
@@ -351,9 +350,7 @@ quant_rows_kernel(Rows r, QuantCache cache) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) mfma_settle(o[t][dt]);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) so[w][16 * dt + 4 * g + i][16 * t + c] = o[t][dt][i];
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(&so[w][16 * t + c][16 * dt + 4 * g]) = o[t][dt];
   }
   __syncthreads();
   const long base = ((long)blockIdx.y * Hkv + kvh) * (16 * NC);
@@ -369,8 +366,9 @@ quant_rows_kernel(Rows r, QuantCache cache) {
     for (int k = 0; k < RW; ++k) {
       const float f = __builtin_amdgcn_exp2f(sm[k][col] - use);
       sum += sl[k][col] * f;
+      const f32x4 y = *reinterpret_cast<const f32x4*>(&so[k][col][d]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += so[k][d + i][col] * f;
+      for (int i = 0; i < 4; ++i) v[i] += y[i] * f;
     }
     if (parts > 1) {
       r.po[(base + col) * (D / 4) + d / 4] = v;
@@ -446,20 +444,20 @@ quant_rows_merge_kernel(Rows r, int Hkv) {
 }  // namespace
 
 // n sequences (list names them, or the first n; list entries and `sequences` bound them), each with at most 16 * tiles rows (query,
-// head of a kv head); per: units of 64 keys a part (0: all over 2^shift workgroups, `least` at least); parts: that many at most, n alone if no sequence
+// head of a kv head); per: units of 64 keys a part (0: all over `share` workgroups, `least` at least); parts: that many at most, n alone if no sequence
 // is cut; ws (parts > n): parts * Hkv * 16 * tiles * (D + 2) floats, then 2 ints for every sequence.
 EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
                            const void* vs, long codes, long scales, int pages, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
                            const int* list, int n, float scale, int Hq, int Hkv, int D, int bs, int causal, int window, int chunk,
-                           int tiles, int parts, int per, int least, int shift, float* ws, hipStream_t st) {
+                           int tiles, int parts, int per, int least, int share, float* ws, hipStream_t st) {
   if (n < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || parts < n || pages < 0 || width < 0 || (parts > n && !ws) || parts > 65535 ||
-      per < 0 || least < 1 || shift < 0 || shift > 24 || tiles < 1)
+      per < 0 || least < 1 || share < 1 || tiles < 1)
     return EIA_BAD_SHAPE;
   if (n == 0) return EIA_OK;
   const int groups = bs / QUANT_GROUP;
   const long rows = (long)parts * Hkv * 16 * tiles;
   Rows r{(const bf16_t*)q, (bf16_t*)out, q_stride, out_stride, tables, lens, cu, list, bt_stride, n, Hq, causal, window, chunk,
-         scale * FLASH_LOG2E, nullptr, nullptr, nullptr, per, least, shift, groups, parts,
+         scale * FLASH_LOG2E, nullptr, nullptr, nullptr, per, least, share, groups, parts,
          pages ? (int)std::min<long>((long)width * bs, INT_MAX) : 0, pages ? pages - 1u : 0u,
          (unsigned)(((1ull << 32) + groups - 1) / groups)};
   if (parts > n) {

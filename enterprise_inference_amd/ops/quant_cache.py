@@ -298,42 +298,54 @@ def _row_tiles(rows: int, head_dim: int) -> int:
     return tiles if 1 <= tiles <= (1 if head_dim == 256 else 2) else 0
 
 
-ROW_SHIFT = 9                 # 2^9 workgroups share out a launch of the few-rows kernel: two a CU
+ROW_SHARE = 512               # workgroups that share out a launch of the few-rows kernel: two a CU, or by _row_share
+ROW_HELD = {(1, 64): 1024, (2, 64): 768, (1, 128): 768, (2, 128): 512, (1, 256): 512}     # (row tiles, D): what the chip holds of them
 ROW_LEAST = 4                 # units a part at least: one a wave
 ROW_LONG = 48                 # longer parts are halved
 
 
-def _launch_rows(name, q, out, cache, block_tables, seq_lens, cu, seqs, n, sequences, scale, causal, window, chunk, tiles, parts, per):
+def _launch_rows(name, q, out, cache, block_tables, seq_lens, cu, seqs, n, sequences, scale, causal, window, chunk, tiles, parts, per,
+                 share):
     Hq, D, device = q.shape[1], cache.head_dim, cache.device
     ws = torch.empty_strided((parts * cache.num_kv_heads * 16 * tiles * (D + 2) + 2 * sequences,), (1,), dtype=torch.float32,
                              device=device) if parts > n else None
     _launch(name, lib().eia_quant_rows, device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *cache._args,
             cache.pages, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu, seqs, n, float(scale), Hq,
-            cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, ROW_SHIFT,
+            cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, share,
             ptr(ws))
 
 
-def _rows_per(units: int) -> int:
+def _row_share(n: int, num_kv_heads: int, tiles: int, head_dim: int) -> int:
+    """Workgroups to share out n sequences over: as many as run at a time, without those that rounding adds (half a part a sequence
+    and head).  us shared over 512 / so, decode, 32 heads on 8 of 128: 32 rows of 8192 to 16384 keys 143 / 138, 15 of 3209 to 6418 39.4 /
+    34.2, 4 of 8301 to 16602 32.1 / 28.5, of 2483 to 4966 14.2 / 14.9, 65 of 1000 to 2000 42.9 / 43.0; 12 on 4 of 256, 32 of 2000 to 4000
+    51.9 / 44.1; chunks of 6 tokens, 32 on 8 of 128, 16 behind 1000 to 2000 27.4 / 21.4; 63 rows of 912, 12 heads of 64, 18.6 / 19.9."""
+    return max(ROW_SHARE // 2, ROW_HELD.get((tiles, head_dim), ROW_SHARE) - n * num_kv_heads // 2)
+
+
+def _rows_per(units: int, share: int = ROW_SHARE) -> int:
     """Units a part for so many of all sequences and kv heads (rows_per in csrc/kernels/quant_rows.hip)."""
-    one = (units + (1 << ROW_SHIFT) - 1) >> ROW_SHIFT
+    one = -(-units // share)
     return max(ROW_LEAST, min(one, max((one + 1) // 2, ROW_LONG)))
 
 
-def _row_parts(n: int, units: int, num_kv_heads: int) -> int:
+def _row_parts(n: int, units: int, num_kv_heads: int, share: int = ROW_SHARE) -> int:
     """Room for the parts of n sequences of at most ``units`` each, whatever their lengths: below one per ``least`` units, and
     fewer than n more than the workgroups that the units are shared out over."""
-    rounds = 2 if n * units * num_kv_heads > ROW_LONG << ROW_SHIFT else 1
-    return min(n * max(1, -(-units // ROW_LEAST)), (rounds << ROW_SHIFT) // num_kv_heads + n)
+    rounds = 2 if n * units * num_kv_heads > ROW_LONG * share else 1
+    return min(n * max(1, -(-units // ROW_LEAST)), rounds * share // num_kv_heads + n)
 
 
 @functools.lru_cache(maxsize=256)
-def _decode_grid(B: int, span: int, group: int, num_kv_heads: int, head_dim: int, window, chunk) -> Tuple[int, int]:
-    """(row tiles, room for parts) of B rows of at most ``span`` tokens."""
+def _decode_grid(B: int, span: int, group: int, num_kv_heads: int, head_dim: int, window, chunk) -> Tuple[int, int, int]:
+    """(row tiles, workgroups to share, room for parts) of B rows of at most ``span`` tokens."""
     units = -(-span // UNIT)
     for w in (window, chunk):
         if w:
             units = min(units, -(-w // UNIT) + 1)
-    return _row_tiles(group, head_dim), _row_parts(B, units, num_kv_heads)
+    tiles = _row_tiles(group, head_dim)
+    share = _row_share(B, num_kv_heads, tiles, head_dim)
+    return tiles, share, _row_parts(B, units, num_kv_heads, share)
 
 
 def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
@@ -348,14 +360,15 @@ def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tenso
         rows = [_attend_plain(q[b:b + 1], cache, block_tables[b], int(seq_lens[b]), scale, True, sliding_window, chunk_size) for b in range(B)]
         r = torch.cat(rows).to(q.dtype) if B else q.clone()
         return r if out is None else out.copy_(r)
-    tiles, parts = _decode_grid(B, block_tables.shape[1] * cache.block_size, Hq // cache.num_kv_heads, cache.num_kv_heads, cache.head_dim,
-                                sliding_window, chunk_size)
+    tiles, share, parts = _decode_grid(B, block_tables.shape[1] * cache.block_size, Hq // cache.num_kv_heads, cache.num_kv_heads,
+                                       cache.head_dim, sliding_window, chunk_size)
     if tiles == 0:
         raise ValueError("quant_decode: too many query heads a kv head")
     o = _empty((B, Hq, cache.head_dim), cache.device) if out is None else out
     if B == 0:
         return o
-    _launch_rows("quant_decode", q, o, cache, block_tables, seq_lens, None, None, B, B, scale, True, sliding_window, chunk_size, tiles, parts, 0)
+    _launch_rows("quant_decode", q, o, cache, block_tables, seq_lens, None, None, B, B, scale, True, sliding_window, chunk_size, tiles, parts,
+                 0, share)
     return o
 
 
@@ -427,7 +440,7 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
             blocks.append((max(0, -(-(hi - lo) // UNIT)), s, r, lo))
     if few:
         plan.n_rows = len(few)
-        plan.row_per = _rows_per(sum(units) * num_kv_heads)
+        plan.row_per = _rows_per(sum(units) * num_kv_heads, _row_share(len(few), num_kv_heads, plan.row_tiles, head_dim))
         plan.row_parts = sum(max(1, -(-u // plan.row_per)) for u in units)
     blocks.sort(key=lambda b: -b[0])
     items, merges = [], []
@@ -536,7 +549,8 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
                 1 if plan.causal else 0, window, chunk)
     if plan.n_rows:
         _launch_rows("quant_prefill", q, o, cache, block_tables, seq_lens, cu_q.data_ptr(), base + 32 * (plan.n_items + plan.n_merge),
-                     plan.n_rows, n, scale, plan.causal, window, chunk, plan.row_tiles, plan.row_parts, plan.row_per)
+                     plan.n_rows, n, scale, plan.causal, window, chunk, plan.row_tiles, plan.row_parts,
+                     plan.row_per, 1)
     return o
 
 

@@ -176,6 +176,17 @@ def test_room_for_parts():
         assert sum(max(1, -(-u // per)) for u in units) <= Q._row_parts(n, w, hk)
 
 
+@pytest.mark.parametrize("share", [256, 300, 448])
+def test_room_for_parts_of_fewer_workgroups(share):
+    import random
+    r = random.Random(share)
+    for _ in range(5000):
+        n, hk, w = r.choice([1, 2, 3, 8, 65, 200]), r.choice([1, 2, 3, 4, 8, 12, 40, 600]), r.choice([1, 3, 4, 5, 16, 100, 512, 3001])
+        units = [r.choice([0, 1, w, r.randint(0, w)]) for _ in range(n)]
+        per = Q._rows_per(sum(units) * hk, share)
+        assert sum(max(1, -(-u // per)) for u in units) <= Q._row_parts(n, w, hk, share)
+
+
 def test_pages_of_two_buffers():
     half = 3 * 32 * 65
     buf = torch.zeros(2, 5, half, dtype=torch.uint8)
