@@ -23,7 +23,12 @@ namespace {
 constexpr int FK = 64;               // keys of a tile
 
 template <int D> struct Shape {
-  static constexpr int THREADS = D == 256 ? 256 : 512;    // 256 channels: four waves, one a SIMD (320 registers)
+  // 128 channels: eight waves of 214 registers, two a SIMD, that share a tile's conversion (two workgroups of four waves: 8192 tokens,
+  // 32 heads on 8, 558 -> 607 us).  256: four waves, one a SIMD (500 registers).  64: a tile is half the products, and a workgroup's
+  // waves wait for one another at its end, so two workgroups of four waves take turns (one of eight -> two of four: 12 heads, four of
+  // 900 behind 3000 80.9 -> 59.8 us, one of 2048 30.9 -> 24.7, 16 on 4, 4096 tokens 73.8 -> 62.6, 8192 200 -> 202).
+  static constexpr int THREADS = D == 128 ? 512 : 256;
+  static constexpr int WAVES = D == 64 ? 3 : D == 128 ? 2 : 1;    // a SIMD: what the registers are held to
   static constexpr int ROWS = THREADS / 64 * 32;
   static constexpr int KS = D + 8, VS = FK + 8;           // row strides in LDS: 16 bytes apart from a power of two
   static constexpr int BUF = FK * KS + D * VS;
@@ -73,7 +78,7 @@ EIA_DEV void put_row(bf16_t* op, const f32x16_t& o, float inv) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(Shape<D>::THREADS, 1)
+__global__ void __launch_bounds__(Shape<D>::THREADS, Shape<D>::WAVES)
 quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
   constexpr int NT = Shape<D>::THREADS, KS = Shape<D>::KS, VS = Shape<D>::VS, BUF = Shape<D>::BUF;
   constexpr int PIECES = 4 * D;                            // 16-byte pieces of a tile's keys, and of its values

@@ -398,7 +398,8 @@ class QuantPrefillPlan:
         self.tokens, self.longest = sum(self.q_lens), max(self.kv_lens, default=0)
 
 
-FLASH_ROWS = {64: 256, 128: 256, 256: 128}      # (query, head) rows of a workgroup of csrc/kernels/quant_flash.hip
+FLASH_ROWS = {64: 128, 128: 256, 256: 128}      # (query, head) rows of a workgroup of csrc/kernels/quant_flash.hip
+FLASH_HELD = {64: 2, 128: 1, 256: 1}            # workgroups on a CU
 
 
 def _first_key(at: int, window, chunk) -> int:
@@ -471,7 +472,7 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
 
 # MI355X, us: a tile of 64 keys of a workgroup with the chip full, what a workgroup takes besides, a part's sums written and read.
 # (Tiles of 32 workgroups alone take 1.45, 1.8 and 3.1: clocks fall under load.)
-FLASH_TILE = {64: 1.5, 128: 2.1, 256: 3.2}
+FLASH_TILE = {64: 1.4, 128: 2.1, 256: 3.2}
 FLASH_FIXED = 4.0
 FLASH_PART = {64: 0.02, 128: 0.033, 256: 0.033}
 FLASH_MERGE = 3.0
@@ -491,7 +492,7 @@ def _makespan(sizes: List[int], slots: int, tile: float) -> float:
 def _flash_per(tiles: List[int], num_kv_heads: int, head_dim: int) -> int:
     """Key tiles of a part at most, for blocks of so many tiles (longest first): what makes the launch shortest, a second kernel
     and the parts' sums counted.  The kv heads are alike, so one is laid out on its share of the CUs."""
-    slots, tile = max(1, CUS // num_kv_heads), FLASH_TILE[head_dim]
+    slots, tile = max(1, CUS * FLASH_HELD[head_dim] // num_kv_heads), FLASH_TILE[head_dim]
     longest, work = max(tiles[0], 1), sum(tiles)
     best, took = longest, _makespan(tiles, slots, tile)
     if len(tiles) >= 4 * slots:                   # many rounds: they even themselves out

@@ -135,7 +135,7 @@ def test_attention(causal, window, chunk):
 def test_work_lists(heads, hk, d, q_lens, lens, causal, window):
     """Every key tile that a block of rows sees lies in one part, parts have places of their own, every row is in one block."""
     plan = Q.quant_prefill_plan(q_lens, lens, heads, hk, d, "cpu", causal, window or None)
-    flat, G, R = plan.lists.tolist(), heads // hk, 128 if d == 256 else 256
+    flat, G, R = plan.lists.tolist(), heads // hk, Q.FLASH_ROWS[d]
     items = [flat[8 * i:8 * i + 5] for i in range(plan.n_items)]
     at = 8 * plan.n_items
     merges = [flat[at + 8 * i:at + 8 * i + 5] for i in range(plan.n_merge)]

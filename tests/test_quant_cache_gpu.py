@@ -578,3 +578,9 @@ def test_more_decode_rows_than_lanes():
     q = torch.randn(130, 8, 128, generator=g).to(BF)
     got = Q.quant_decode(q.cuda(), _on_gpu(parts), bt.cuda(), _i32(lens), 0.02)
     C.check_attention(got.cpu(), *C.attend64(q, parts, bt, [1] * 130, lens, 0.02))
+
+
+def test_blocks_of_plan_and_kernel():
+    Q = _q()
+    from enterprise_inference_amd.ops._dispatch import lib
+    assert {d: lib().eia_quant_flash_rows(d) for d in Q.HEAD_DIMS} == Q.FLASH_ROWS
