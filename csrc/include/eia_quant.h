@@ -45,6 +45,13 @@ EIA_DEV unsigned quant_byte(unsigned amax_bits) {
 }
 EIA_DEV float quant_inverse(unsigned byte) { return __uint_as_float((254 - byte) << 23); }    // 2^-e, byte in [27, 246]
 
+// A double as the float on its way to a code: cut off, and its last bit set if anything was, so that the nearest code of the float is
+// that of the double (rounded to the nearest twice, a value beside a border would come to lie on it: one key in a million.  4096 tokens 20.4 -> 20.8 us).
+EIA_DEV float quant_odd(double x) {
+  const unsigned hi = (unsigned)__double2hiint(x), lo = (unsigned)__double2loint(x);
+  return (float)__hiloint2double((int)hi, (int)((lo & 0xe0000000u) | (min(lo << 3, 1u) << 29)));
+}
+
 // Four values, scaled, as codes.  Nothing scaled passes 448 but rows beyond 448 * 2^119.
 EIA_DEV unsigned quant_pack(float a, float b, float c, float d, float inv) {
   auto held = [&](float x) { return fminf(fmaxf(x * inv, -448.f), 448.f); };

@@ -66,8 +66,8 @@ template <int D, bool NEOX, bool ONCE> struct RowLoad {
   }
 };
 
-// T: queries are rounded to bf16 and formed in fp32; keys in fp64 (their codes are borders apart, and the heads are few): what
-// a code is the nearest to is then off by fp32's last rounding alone.
+// T: queries are rounded to bf16 and formed in fp32; keys in fp64 (their codes are borders apart, and the heads are few), so that a code
+// is the nearest to what bias, norm and rotation of the projection's numbers give.
 template <int D, bool NEOX, typename T>
 EIA_DEV void norm_row(const bf16_t* w, float eps, int sub, T (&x)[16]) {
   T ss = 0;
@@ -170,7 +170,7 @@ quant_write_kernel(QuantSrc src, const int* __restrict__ positions, const float*
       if (src.k_norm) norm_row<D, NEOX>(src.k_norm, src.eps, sub, x);
       if (cos_sin) turn.template rotate<NEOX>(x);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) k[j] = (float)x[j];
+      for (int j = 0; j < 16; ++j) k[j] = quant_odd(x[j]);
     }
     // magnitudes as bits: what is not finite is the largest
     unsigned mk = 0, mv = 0;

@@ -584,3 +584,32 @@ def test_blocks_of_plan_and_kernel():
     Q = _q()
     from enterprise_inference_amd.ops._dispatch import lib
     assert {d: lib().eia_quant_flash_rows(d) for d in Q.HEAD_DIMS} == Q.FLASH_ROWS
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_codes_are_the_nearest(norm):
+    """A million rotated keys: every code is what rounding the 64-bit value once gives (values so near to a border that 64 bits
+    miss it are some 2^-45 of them)."""
+    Q = _q()
+    from enterprise_inference_amd.ops.rotary import RotaryCache
+    H, hk, D, T, bs = 4, 2, 128, 4096, 128
+    g = torch.Generator(device="cuda").manual_seed(31)
+    rot = RotaryCache(D, 9000, 10000.0, None, torch.device("cuda"))
+    qkv = torch.randn(T, (H + 2 * hk) * D, generator=g, device="cuda").to(BF)
+    pos, slots = torch.randint(0, 9000, (T,), generator=g, device="cuda").to(torch.int32), torch.arange(T, device="cuda", dtype=torch.int32)
+    w = (1 + 0.2 * torch.randn(D, generator=g, device="cuda")).to(BF) if norm else None
+    cache = Q.QuantKVCache.allocate(T // bs, hk, bs, D, "cuda")
+    Q.rope_qkv_quant(qkv, pos, rot, slots, cache, H, hk, D, None, w, w)
+    x = qkv.view(T, H + 2 * hk, D)[:, H:H + hk].double()
+    if norm:
+        x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+    c, s = rot.cos_sin[pos.long()].double().unsqueeze(1).chunk(2, -1)
+    a, b = x.chunk(2, -1)
+    x = torch.cat([a * c - b * s, b * c + a * s], -1)
+    two_to = lambda n: ((n.long() + 1023) << 52).view(torch.float64)            # (torch.ldexp takes a power of 2.0, which is not exact)
+    mant, e = torch.frexp(x.abs().amax(-1, keepdim=True))
+    e = e - 9 + (mant > 0.875).int()
+    y = x * two_to(-e)
+    step = two_to(torch.frexp(y)[1].clamp(min=-5) - 4)
+    want = torch.round(y / step) * step * two_to(e)
+    assert torch.equal(Q.quant_read(cache, slots)[0].double(), want)
