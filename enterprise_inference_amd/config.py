@@ -363,6 +363,13 @@ class EngineConfig:
                                  "for those that lay out their own")
             if self.model.head_dim not in (64, 128, 256):
                 raise ValueError(f"the 8-bit KV cache takes heads of 64, 128 or 256, not {self.model.head_dim}")
+            if self.cache.block_size % 16:
+                raise ValueError(f"the 8-bit KV cache takes blocks of a multiple of 16 tokens, not {self.cache.block_size}")
+            tp = self.parallel.tensor_parallel_size
+            group = self.model.num_attention_heads // tp // max(1, self.model.num_key_value_heads // tp)
+            most = 16 if self.model.head_dim == 256 else 32
+            if group > most:
+                raise ValueError(f"the 8-bit KV cache takes {most} query heads a KV head of {self.model.head_dim}, not {group}")
         if self._model_attr("needs_state_slots") and not self.cache.num_state_slots:
             self.cache.num_state_slots = self.scheduler.max_num_seqs
         if self.scheduler.max_model_len > self.model.max_position_embeddings and \

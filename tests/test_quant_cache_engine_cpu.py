@@ -68,6 +68,16 @@ def test_what_is_refused():
         EngineConfig(model=cfg, cache=CacheConfig(cache_dtype=torch.float8_e4m3fn), device="cpu", dtype=torch.float32)
 
 
+def test_blocks_and_groups_that_are_refused():
+    def config(heads, d, block=128):
+        cfg = ModelConfig.from_hf_dict(_config("LlamaForCausalLM") | dict(num_attention_heads=heads, num_key_value_heads=1, head_dim=d))
+        return EngineConfig(model=cfg, cache=CacheConfig(cache_dtype=torch.float8_e4m3fn, block_size=block), device="cpu", dtype=torch.float32)
+    config(32, 128), config(16, 256), config(4, 64, 48)
+    for args, what in (((33, 128), "query heads"), ((17, 256), "query heads"), ((4, 64, 40), "multiple of 16")):
+        with pytest.raises(ValueError, match=what):
+            config(*args)
+
+
 def test_command_line(tmp_path):
     import json
 
