@@ -16,8 +16,10 @@
 // 32 heads on 8 of 128, 32 rows of 8192 to 16384 keys 137 us, 6.1 TB/s (a kernel that only reads reaches 6.4); 65 of 1000 to 2000 42 us,
 // 4.6 TB/s, parts that do not come out even.  Short launches are a chain of waits: lengths, table, keys, a unit or two a wave (2.4 us each
 // with two column tiles), the waves' sums, the merge's launch: one row of 4000 keys 8.8 us in a graph.
-// Four waves take every fourth unit and meet once at the end.  Two, and twice the workgroups: 65 rows 42.8 -> 40.9, but one of 28749 on 4
-// heads 17.9 -> 22.3, and 7 % slower over 64 cases.  Meeting inside the kernel, the last part to arrive merging: one row 9.3 -> 9.9.
+// Four waves (RW) take every fourth unit and meet once at the end, or two every second, where there are more rows and heads than the chip holds
+// workgroups of four (what these are for, short chains, is gone then).  32 heads on 8 of 128, us with four / two: 128 rows of 65 to 130 keys 14.5 /
+// 12.3, of 250 to 500 30.6 / 27.4, of 1000 to 2000 79.2 / 72.8, 100 of 1000 to 2000 62.1 / 63.9; below that, 90 rows of 500 to 1000 33.2 /
+// 38.1, one of 28749 on 4 heads 17.9 / 22.3.  Meeting inside the kernel, the last part to arrive merging: one row 9.3 -> 9.9.
 #include <algorithm>
 #include <climits>
 
@@ -27,7 +29,6 @@
 namespace {
 
 constexpr int RU = 64;               // keys a wave takes at a time
-constexpr int RW = 4;                // waves of a workgroup
 
 struct Rows {
   const bf16_t* q;
@@ -134,7 +135,7 @@ EIA_DEV void put_rows(const Rows& r, int q0, int kvh, int G, int D, int col, int
   *reinterpret_cast<bf16x4*>(r.out + (long)(q0 + col / G) * r.out_stride + (long)(kvh * G + col % G) * D + d) = y;
 }
 
-template <int D, int NC, bool UNI>
+template <int D, int NC, bool UNI, int RW>
 __global__ void __launch_bounds__(64 * RW, D == 256 || NC == 2 ? 2 : D == 128 ? 3 : 4)
 quant_rows_kernel(Rows r, QuantCache cache) {
   constexpr int KC = D / 64;         // 16-byte pieces of a key row a lane holds
@@ -451,14 +452,14 @@ quant_rows_merge_kernel(Rows r, int Hkv) {
 }  // namespace
 
 // n sequences (list names them, or the first n; list entries and `sequences` bound them), each with at most 16 * tiles rows (query,
-// head of a kv head); per: units of 64 keys a part (0: all over `share` workgroups, `least` at least); parts: that many at most, n alone if no sequence
+// head of a kv head); per: units of 64 keys a part (0: all over `share` workgroups, `least` at least); waves of a workgroup: 4, or 2 (one tile, D <= 128); parts: that many at most, n alone if no sequence
 // is cut; ws (parts > n): parts * Hkv * 16 * tiles * (D + 2) floats, then 2 ints for every sequence.
 EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_stride, const void* k, const void* v, const void* ks,
                            const void* vs, long codes, long scales, int pages, const int* tables, int bt_stride, int width, const int* lens, const int* cu,
                            const int* list, int n, float scale, int Hq, int Hkv, int D, int bs, int causal, int window, int chunk,
-                           int tiles, int parts, int per, int least, int share, float* ws, hipStream_t st) {
+                           int tiles, int parts, int per, int least, int share, int waves, float* ws, hipStream_t st) {
   if (n < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || bs <= 0 || bs % QUANT_GROUP || parts < n || pages < 0 || width < 0 || (parts > n && !ws) || parts > 65535 ||
-      per < 0 || least < 1 || share < 1 || tiles < 1)
+      per < 0 || least < 1 || share < 1 || (waves != 4 && (waves != 2 || tiles > 1 || D > 128)) || tiles < 1)
     return EIA_BAD_SHAPE;
   if (n == 0) return EIA_OK;
   const int groups = bs / QUANT_GROUP;
@@ -475,10 +476,18 @@ EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_str
     r.per = 1 << 30;
   }
   const QuantCache c{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, codes, scales, Hkv, bs};
+#define RW_ROWS(D, NC, W)                                                                                                     \
+  do {                                                                                                                        \
+    if (bs % RU == 0) hipLaunchKernelGGL((quant_rows_kernel<D, NC, true, W>), dim3(Hkv, parts), dim3(64 * W), 0, st, r, c);   \
+    else hipLaunchKernelGGL((quant_rows_kernel<D, NC, false, W>), dim3(Hkv, parts), dim3(64 * W), 0, st, r, c);               \
+  } while (0)
 #define RW_GO(D, NC)                                                                                                      \
   do {                                                                                                                    \
-    if (bs % RU == 0) hipLaunchKernelGGL((quant_rows_kernel<D, NC, true>), dim3(Hkv, parts), dim3(64 * RW), 0, st, r, c); \
-    else hipLaunchKernelGGL((quant_rows_kernel<D, NC, false>), dim3(Hkv, parts), dim3(64 * RW), 0, st, r, c);             \
+    if constexpr (NC == 1 && D <= 128) {                                                                                  \
+      if (waves == 2) RW_ROWS(D, NC, 2); else RW_ROWS(D, NC, 4);                                                          \
+    } else {                                                                                                              \
+      RW_ROWS(D, NC, 4);                                                                                                  \
+    }                                                                                                                     \
     if (parts > n)                                                                                                        \
       hipLaunchKernelGGL((quant_rows_merge_kernel<D, NC>), dim3(Hkv, n, cu ? 16 * NC : Hq / Hkv), dim3(256), 0, st, r, Hkv); \
   } while (0)
@@ -490,5 +499,6 @@ EIA_API int eia_quant_rows(const void* q, long q_stride, void* out, long out_str
     default: return EIA_UNSUPPORTED;
   }
 #undef RW_GO
+#undef RW_ROWS
   EIA_LAUNCH_CHECK();
 }

@@ -47,7 +47,7 @@ _SIGNATURES = {
     "eia_paged_prefill_fa": [P, L, P, L, P, P, IP, I, IP, IP, IP, I, F, I, I, I, I, I, I, I, I, I, P, S],
     "eia_quant_write": [P, L, P, I, IP, P, I, IP, P, P, P, P, L, L, I, P, P, P, P, F, I, I, I, I, I, I, S],
     "eia_quant_read": [P, P, P, P, L, L, I, IP, I, P, P, I, I, I, S],
-    "eia_quant_rows": [P, L, P, L, P, P, P, P, L, L, I, IP, I, I, IP, IP, IP, I, F, I, I, I, I, I, I, I, I, I, I, I, I, P, S],
+    "eia_quant_rows": [P, L, P, L, P, P, P, P, L, L, I, IP, I, I, IP, IP, IP, I, F, I, I, I, I, I, I, I, I, I, I, I, I, I, P, S],
     "eia_quant_flash": [P, L, P, L, P, P, P, P, L, L, I, IP, I, I, IP, I, IP, I, I, P, F, I, I, I, I, I, I, I, S],
     "eia_quant_flash_rows": [I],
     "eia_act_and_mul": [P, P, I, I, L, L, I, S],

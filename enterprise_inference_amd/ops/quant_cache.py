@@ -300,7 +300,7 @@ def _row_tiles(rows: int, head_dim: int) -> int:
 
 ROW_SHARE = 512               # workgroups that share out a launch of the few-rows kernel: two a CU, or by _row_share
 ROW_HELD = {(1, 64): 1024, (2, 64): 768, (1, 128): 768, (2, 128): 512, (1, 256): 512}     # (row tiles, D): what the chip holds of them
-ROW_LEAST = 4                 # units a part at least: one a wave
+ROW_LEAST = 4                 # units a part at least
 ROW_LONG = 48                 # longer parts are halved
 
 
@@ -311,16 +311,19 @@ def _launch_rows(name, q, out, cache, block_tables, seq_lens, cu, seqs, n, seque
                              device=device) if parts > n else None
     _launch(name, lib().eia_quant_rows, device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *cache._args,
             cache.pages, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), cu, seqs, n, float(scale), Hq,
-            cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, share,
+            cache.num_kv_heads, D, cache.block_size, 1 if causal else 0, window or 0, chunk or 0, tiles, parts, per, ROW_LEAST, *share,
             ptr(ws))
 
 
-def _row_share(n: int, num_kv_heads: int, tiles: int, head_dim: int) -> int:
-    """Workgroups to share out n sequences over: as many as run at a time, without those that rounding adds (half a part a sequence
-    and head).  us shared over 512 / so, decode, 32 heads on 8 of 128: 32 rows of 8192 to 16384 keys 143 / 138, 15 of 3209 to 6418 39.4 /
+def _row_share(n: int, num_kv_heads: int, tiles: int, head_dim: int) -> Tuple[int, int]:
+    """(Workgroups to share out n sequences over, waves of one): as many as run at a time, without those that rounding adds (half a part a
+    sequence and head).  us shared over 512 / so, decode, 32 heads on 8 of 128: 32 rows of 8192 to 16384 keys 143 / 138, 15 of 3209 to 6418 39.4 /
     34.2, 4 of 8301 to 16602 32.1 / 28.5, of 2483 to 4966 14.2 / 14.9, 65 of 1000 to 2000 42.9 / 43.0; 12 on 4 of 256, 32 of 2000 to 4000
-    51.9 / 44.1; chunks of 6 tokens, 32 on 8 of 128, 16 behind 1000 to 2000 27.4 / 21.4; 63 rows of 912, 12 heads of 64, 18.6 / 19.9."""
-    return max(ROW_SHARE // 2, ROW_HELD.get((tiles, head_dim), ROW_SHARE) - n * num_kv_heads // 2)
+    51.9 / 44.1; chunks of 6 tokens, 32 on 8 of 128, 16 behind 1000 to 2000 27.4 / 21.4.  Workgroups of two waves where the heads and rows
+    alone are more than that (csrc/kernels/quant_rows.hip has the times)."""
+    held, alone = ROW_HELD.get((tiles, head_dim), ROW_SHARE), n * num_kv_heads
+    two = tiles == 1 and head_dim <= 128 and alone > held
+    return max(ROW_SHARE // 2, (held * 3 // 2 if two else held) - alone // 2), 2 if two else 4
 
 
 def _rows_per(units: int, share: int = ROW_SHARE) -> int:
@@ -337,15 +340,15 @@ def _row_parts(n: int, units: int, num_kv_heads: int, share: int = ROW_SHARE) ->
 
 
 @functools.lru_cache(maxsize=256)
-def _decode_grid(B: int, span: int, group: int, num_kv_heads: int, head_dim: int, window, chunk) -> Tuple[int, int, int]:
-    """(row tiles, workgroups to share, room for parts) of B rows of at most ``span`` tokens."""
+def _decode_grid(B: int, span: int, group: int, num_kv_heads: int, head_dim: int, window, chunk) -> Tuple[int, Tuple[int, int], int]:
+    """(row tiles, workgroups to share and their waves, room for parts) of B rows of at most ``span`` tokens."""
     units = -(-span // UNIT)
     for w in (window, chunk):
         if w:
             units = min(units, -(-w // UNIT) + 1)
     tiles = _row_tiles(group, head_dim)
     share = _row_share(B, num_kv_heads, tiles, head_dim)
-    return tiles, share, _row_parts(B, units, num_kv_heads, share)
+    return tiles, share, _row_parts(B, units, num_kv_heads, share[0])
 
 
 def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
@@ -391,6 +394,7 @@ class QuantPrefillPlan:
     row_tiles: int = 1
     row_parts: int = 1
     row_per: int = 0
+    row_waves: int = 4
 
     stream = ready = None                  # of the lists' upload
 
@@ -441,7 +445,8 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
             blocks.append((max(0, -(-(hi - lo) // UNIT)), s, r, lo))
     if few:
         plan.n_rows = len(few)
-        plan.row_per = _rows_per(sum(units) * num_kv_heads, _row_share(len(few), num_kv_heads, plan.row_tiles, head_dim))
+        share, plan.row_waves = _row_share(len(few), num_kv_heads, plan.row_tiles, head_dim)
+        plan.row_per = _rows_per(sum(units) * num_kv_heads, share)
         plan.row_parts = sum(max(1, -(-u // plan.row_per)) for u in units)
     blocks.sort(key=lambda b: -b[0])
     items, merges = [], []
@@ -551,7 +556,7 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
     if plan.n_rows:
         _launch_rows("quant_prefill", q, o, cache, block_tables, seq_lens, cu_q.data_ptr(), base + 32 * (plan.n_items + plan.n_merge),
                      plan.n_rows, n, scale, plan.causal, window, chunk, plan.row_tiles, plan.row_parts,
-                     plan.row_per, 1)
+                     plan.row_per, (1, plan.row_waves))
     return o
 
 

@@ -613,3 +613,32 @@ def test_codes_are_the_nearest(norm):
     step = two_to(torch.frexp(y)[1].clamp(min=-5) - 4)
     want = torch.round(y / step) * step * two_to(e)
     assert torch.equal(Q.quant_read(cache, slots)[0].double(), want)
+
+
+@pytest.mark.parametrize("H,hk,D,bs,B", [(32, 8, 128, 64, 100), (12, 12, 64, 48, 90), (16, 16, 128, 16, 70)])
+def test_more_rows_and_heads_than_run_at_a_time(H, hk, D, bs, B):
+    Q = _q()
+    assert Q._row_share(B, hk, 1, D)[1] == 2 and Q._row_share(B // 2, hk, 1, D)[1] == 4
+    g = torch.Generator().manual_seed(B)
+    lens = [int(x) for x in torch.randint(0, 200, (B,), generator=g)]
+    lens[3], lens[4], lens[B - 1] = 2900, 0, 64
+    bt, pages = C.tables(g, lens, bs)
+    parts = C.raw_cache(g, pages, hk, bs, D)
+    C.spoil_behind(parts, bt, lens, bs)
+    q = torch.randn(B, H, D, generator=g).to(BF)
+    args = _on_gpu(parts), bt.cuda(), _i32(lens), 0.02
+    got = Q.quant_decode(q.cuda(), *args)
+    for s in (0, 1, 2, 3, 4, 5, B - 2, B - 1):
+        if lens[s]:
+            C.check_attention(got[s:s + 1].cpu(), *_dense64(q[s:s + 1].cuda(), parts, bt[s], lens[s], 1))
+        else:
+            assert not got[s].any()
+    # chunks of two tokens, the same rule
+    plan = Q.quant_prefill_plan([1, 2] * (B // 2), lens, H, hk, D, "cuda")
+    assert plan.row_waves == 2 and plan.n_rows == B
+    cu = _i32([0] + [1, 2] * (B // 2)).cumsum(0).to(torch.int32)
+    q2 = torch.randn(int(cu[-1]), H, D, generator=g).to(BF).cuda()
+    got = Q.quant_prefill(q2, *args[:3], cu, plan, 0.02)
+    for s in (1, 3, B - 1):
+        a = int(cu[s])
+        C.check_attention(got[a:a + 2].cpu(), *_dense64(q2[a:a + 2], parts, bt[s], lens[s], 2))
