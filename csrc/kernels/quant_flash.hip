@@ -13,14 +13,17 @@
 // The host lays the launch out (which rows, which tiles): blocks that would be the launch's tail are cut along the keys,
 // their parts hand over fp32 sums and a second kernel puts them together.
 //
-// Bound by issue: 128 channels, of the 4380 cycles that two waves of a SIMD take for a tile each the matrix unit works in 2048 and the
-// vector unit in some 2900 (exponentials, maxima, packing, conversion), LDS in 2300; they overlap by half.  8192 tokens, 32
-// heads on 8: 555 us, 990 TFLOP/s of the causal half, where a plain bf16 product of 8192^3 reaches 1281.  256 channels: 515 TFLOP/s (4096
+// Bound by issue, and by power: 128 channels, of the 4300 cycles that two waves of a SIMD take for a tile each the matrix unit works in 2048 and
+// the vector unit in some 2900 (exponentials, maxima, packing, conversion), LDS in 2300.  The halves of a workgroup take turns (by the
+// clock, with its reads in the way: scores and conversion 1100 to 1300, outputs 670; codes asked for 400 to 600, weights 1400), 555 -> 544 us
+// at 8192 tokens, 32 heads on 8; clocks fall from 2.2 to 2.0 GHz as the units fill.  1010 TFLOP/s of the causal half, where a plain bf16
+// product of 8192^3 reaches 1281.  256 channels: 515 TFLOP/s (4096
 // tokens, 12 heads on 4), one wave a SIMD, whose products wait for its own vector work; 64: 680 (8192, 16 on 4), exponentials.
 // Measured and left: 64 rows a wave 732 us; the next tile's first product beside this one's exponentials 550 for 547; fp8 products
 // with queries as two codes 527 for 542, but 4 us more in short launches and scores that lose their last bits.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "eia_flash.h"
 #include "eia_quant.h"
@@ -38,7 +41,9 @@ template <int D> struct Shape {
   static constexpr int WAVES = D == 64 ? 3 : D == 128 ? 2 : 1;    // a SIMD: what the registers are held to
   static constexpr int ROWS = THREADS / 64 * 32;
   static constexpr int KS = D + 8, VS = FK + 8;           // row strides in LDS: 16 bytes apart from a power of two
-  static constexpr int BUF = FK * KS + D * VS;
+  static constexpr bool TURNS = THREADS == 512;           // halves of the workgroup multiply and weigh in turn
+  static constexpr int NV = TURNS ? 3 : 2;                // value tiles in LDS
+  static constexpr int LDS = 2 * FK * KS + NV * D * VS;
 };
 
 // A block of rows of a sequence (its first query, queries and keys): first row, first key, key tiles, place of a part's sums (-1:
@@ -87,13 +92,15 @@ EIA_DEV void put_row(bf16_t* op, const f32x16_t& o, float inv) {
 template <int D>
 __global__ void __launch_bounds__(Shape<D>::THREADS, Shape<D>::WAVES)
 quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
-  constexpr int NT = Shape<D>::THREADS, KS = Shape<D>::KS, VS = Shape<D>::VS, BUF = Shape<D>::BUF;
+  constexpr int NT = Shape<D>::THREADS, KS = Shape<D>::KS, VS = Shape<D>::VS, NV = Shape<D>::NV;
+  constexpr bool TURNS = Shape<D>::TURNS;
   constexpr int PIECES = 4 * D;                            // 16-byte pieces of a tile's keys, and of its values
   constexpr bool SHARED = PIECES < NT;                     // half the threads take keys, half values
   constexpr int NP = SHARED ? 1 : PIECES / NT;
   static_assert(!SHARED || 2 * PIECES == NT, "");
-  __shared__ __align__(16) bf16_t lds[2 * BUF];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r32 = lane & 31, h = lane >> 5;
+  __shared__ __align__(16) bf16_t lds[Shape<D>::LDS];
+  bf16_t* const vlds = lds + 2 * FK * KS;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, h = lane >> 5;
   const Item it = items[blockIdx.y];
   const int kvh = blockIdx.x, Hkv = cache.Hkv, G = a.Hq / Hkv;
   const int qbeg = it.qbeg, qlen = it.qlen, L = min(it.len, a.longest), ctx = L - qlen;
@@ -170,9 +177,9 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     }
   };
   // Half h of a thread's pieces, converted, into LDS.
-  auto stash = [&](int buf, int i, int h) {
-    bf16_t* kl = lds + buf * BUF;
-    bf16_t* vl = kl + FK * KS;
+  auto stash = [&](int kbuf, int vbuf, int i, int h) {
+    bf16_t* kl = lds + kbuf * (FK * KS);
+    bf16_t* vl = vlds + vbuf * (D * VS);
     const int id = piece(i);
     if (keys_here) {
       bf16_t* p = kl + id / (D / 16) * KS + 16 * (id % (D / 16)) + 8 * h;
@@ -193,11 +200,11 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
       *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   };
-  auto stash_all = [&](int buf) {
+  auto stash_all = [&](int kbuf, int vbuf) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      stash(buf, i, 0);
-      stash(buf, i, 1);
+      stash(kbuf, vbuf, i, 0);
+      stash(kbuf, vbuf, i, 1);
     }
   };
 
@@ -215,24 +222,23 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
       if (t + 3 < it.tiles) look(t + 3);
     }
   };
-  auto compute = [&](int t, int kb) {
-    const int buf = t & 1;
-    const bf16_t* kf0 = lds + buf * BUF + krow * KS + 8 * h;
-    const bf16_t* vf0 = lds + buf * BUF + FK * KS + r32 * VS + 8 * h;
-    f32x16_t sc[2];
-    // reads of LDS go four fragments ahead of the products; products go before the other wave's vector work
+  f32x16_t sc[2];
+  bf16x8 p[4];
+  float sum[4];
+  // scores of tile t; beside them tile t + 1 is converted.  Reads of LDS go four fragments ahead of the products
+  auto scores = [&](int t, int vbuf) {
+    const bf16_t* kf0 = lds + (t & 1) * (FK * KS) + krow * KS + 8 * h;
     bf16x8 kf[2][4];
     auto keys = [&](int b) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) kf[b & 1][x] = *reinterpret_cast<const bf16x8*>(kf0 + 32 * KS * (x & 1) + 16 * (2 * b + (x >> 1)));
     };
-    __builtin_amdgcn_s_setprio(1);
     keys(0);
 #pragma unroll
     for (int b = 0; b < D / 32; ++b) {
       if (b + 1 < D / 32) keys(b + 1);
       __builtin_amdgcn_sched_barrier(0);
-      if (b < 2 * NP) stash(buf ^ 1, b >> 1, b & 1);
+      if (b < 2 * NP) stash((t + 1) & 1, vbuf, b >> 1, b & 1);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int step = 2 * b + (x >> 1);
@@ -240,9 +246,10 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
-    ahead(t);
-    // element i of half sh is key kb + 32 sh + 16 (i / 8) + 8 h + i % 8
+  };
+  // the tile's mask and maximum: element i of half sh is key kb + 32 sh + 16 (i / 8) + 8 h + i % 8
+  float use;
+  auto bound = [&](int kb) {
     const bool whole = !window && kb + FK <= L && (!a.causal || kb + FK - 1 <= ctx + wq0);
     mfma_settle(sc[0], sc[1]);
     if (!whole) {
@@ -271,45 +278,45 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) o[dt] *= old;
     }
-    const float use = m == -INFINITY ? 0.f : m;
-    bf16x8 p[4];
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    auto weights = [&](int ks) {
+    use = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const f32x16_t& v = sc[ks >> 1];
-        const int e = 8 * (ks & 1) + j;
-        const bf16x2 y = flash_pack(__builtin_amdgcn_exp2f(fmaf(v[e], a.scale_log2, -use)), __builtin_amdgcn_exp2f(fmaf(v[e + 1], a.scale_log2, -use)));
-        p[ks][j] = y[0];
-        p[ks][j + 1] = y[1];
-        sum[ks] = __builtin_amdgcn_fdot2_f32_bf16(y, bf16x2{(bf16_t)1.f, (bf16_t)1.f}, sum[ks], false);
-      }
-    };
-    constexpr int VB = D / 32 < 4 ? D / 32 : 4;            // fragments of values read ahead
+    for (int c = 0; c < 4; ++c) sum[c] = 0.f;
+  };
+  auto weights = [&](int ks) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const f32x16_t& v = sc[ks >> 1];
+      const int e = 8 * (ks & 1) + j;
+      const bf16x2 y = flash_pack(__builtin_amdgcn_exp2f(fmaf(v[e], a.scale_log2, -use)), __builtin_amdgcn_exp2f(fmaf(v[e + 1], a.scale_log2, -use)));
+      p[ks][j] = y[0];
+      p[ks][j + 1] = y[1];
+      sum[ks] = __builtin_amdgcn_fdot2_f32_bf16(y, bf16x2{(bf16_t)1.f, (bf16_t)1.f}, sum[ks], false);
+    }
+  };
+  constexpr int VB = D / 32 < 4 ? D / 32 : 4, NB = D / 32 / VB;      // fragments of values read ahead, blocks of channels of them
+  // the outputs of a tile; its weights formed beside the products, or there already
+  auto outputs = [&](int vbuf, auto form) {
+    const bf16_t* vf0 = vlds + vbuf * (D * VS) + r32 * VS + 8 * h;
     bf16x8 vf[2][VB];
-    auto values = [&](int s) {                             // step s: channels of block s % (D / 32 / VB), keys of s / (...)
-      constexpr int NB = D / 32 / VB;
+    auto values = [&](int s) {                             // step s: channels of block s % NB, keys of s / NB
 #pragma unroll
       for (int x = 0; x < VB; ++x) vf[s & 1][x] = *reinterpret_cast<const bf16x8*>(vf0 + 32 * VS * (VB * (s % NB) + x) + 16 * (s / NB));
     };
-    __builtin_amdgcn_s_setprio(2);
     values(0);
     __builtin_amdgcn_sched_barrier(0);
-    weights(0);
-    constexpr int NB = D / 32 / VB;
+    if (form) weights(0);
 #pragma unroll
     for (int s = 0; s < 4 * NB; ++s) {
       if (s + 1 < 4 * NB) {
         values(s + 1);
-        if ((s + 1) % NB == 0) weights((s + 1) / NB);
+        if (form && (s + 1) % NB == 0) weights((s + 1) / NB);
       }
+      if (!form) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < VB; ++x)
         o[VB * (s % NB) + x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s & 1][x], p[s / NB], o[VB * (s % NB) + x], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    __builtin_amdgcn_s_setprio(0);
   };
 
   // Tile t is multiplied while tile t + 1 is converted, beside the first product, and tile t + 2 is on its way.
@@ -318,21 +325,69 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     fetch();
     look(min(1, it.tiles - 1));
     ready(0);
-    stash_all(0);
+    stash_all(0, 0);
     if (it.tiles > 1) fetch();
     if (it.tiles > 2) look(2);
   }
   __syncthreads();
-  for (int t = 0; t < it.tiles; ++t) {
-    const int kb = it.lo + FK * t;
-    ready(t + 1);                                          // (behind the last tile: the same registers into the buffer that nobody reads)
-    if (kb < w_hi && kb + FK > w_lo) {                     // (the same for the wave)
-      compute(t, kb);
-    } else {
-      stash_all((t + 1) & 1);
+  // (behind the last tile the same registers go into a buffer that nobody reads)
+  if constexpr (TURNS) {
+    // Four waves, one on each SIMD, multiply (scores of tile t and the conversion beside it, outputs of tile t - 1) while the other
+    // four form weights and ask for codes; then the halves change places.  Keys of tile t + 1 are stored while both halves may still read those of t, values
+    // while t - 1 is read too: three places.  Every wave passes 2 T + 1 barriers.
+    auto turn = [&] {
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    const bool late = w >= NT / 128;
+    if (late) turn();
+    bool before = false;
+    int was = NV - 1, at = 0;                                // places of the values of tiles t - 1 and t
+    for (int t = 0; t < it.tiles; ++t) {
+      const int kb = it.lo + FK * t, next = at == NV - 1 ? 0 : at + 1;
+      const bool now = kb < w_hi && kb + FK > w_lo;        // (the same for the wave)
+      ready(t + 1);
+      __builtin_amdgcn_s_setprio(1);
+      if (now) scores(t, next);
+      else stash_all((t + 1) & 1, next);
+      if (before) outputs(was, std::false_type{});
+      __builtin_amdgcn_s_setprio(0);
+      turn();
       ahead(t);
+      if (now) {
+        bound(kb);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) weights(ks);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+      turn();
+      before = now;
+      was = at;
+      at = next;
     }
-    __syncthreads();
+    if (before) outputs(was, std::false_type{});
+    if (!late) turn();
+  } else {
+    for (int t = 0; t < it.tiles; ++t) {
+      const int kb = it.lo + FK * t;
+      ready(t + 1);
+      if (kb < w_hi && kb + FK > w_lo) {                   // (the same for the wave)
+        __builtin_amdgcn_s_setprio(1);                     // products go before the other wave's vector work
+        scores(t, (t + 1) & 1);
+        __builtin_amdgcn_s_setprio(0);
+        ahead(t);
+        bound(kb);
+        __builtin_amdgcn_s_setprio(2);
+        outputs(t & 1, std::true_type{});
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        __builtin_amdgcn_s_setprio(0);
+      } else {
+        stash_all((t + 1) & 1, (t + 1) & 1);
+        ahead(t);
+      }
+      __syncthreads();
+    }
   }
 
 #pragma unroll
