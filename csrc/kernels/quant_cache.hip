@@ -1,8 +1,8 @@
 // Writing and reading the 8-bit key/value cache (eia_quant.h).
 //
 // The write takes the QKV projection's rows [T, (Hq + 2 Hkv) D] (bf16, or the fp32 partial sums of a split-K GEMM):
-// bias, RMS norm of queries and keys, rotation; queries go on in bf16, keys and values into the cache.  All of it in
-// fp32, rounded once: a key's code is the nearest to the rotated fp32 value.
+// bias, RMS norm of queries and keys, rotation; queries go on in bf16, keys and values into the cache.  All of it
+// rounded once: queries are formed in fp32, keys in fp64, values are the projection's own and a bias.
 //
 // A head of a token is D / 16 lanes, sixteen values a lane (two halves of eight, as they rotate); the lanes of a kv head
 // hold the key row and the value row, because a value that is not finite marks both.  A workgroup takes TT tokens and

@@ -195,8 +195,8 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
                    k_norm_w: Optional[torch.Tensor] = None, norm_eps: float = 1e-6) -> torch.Tensor:
     """qkv [T, (Hq + 2 Hkv) D] -> q [T, Hq, D]; keys and values go into the 8-bit cache (``rope_qkv_cache`` for it).
 
-    ``qkv`` may be a ``gemm.SplitK``, summed here.  Bias, per-head norms and rotation are fp32, rounded once: queries to bf16,
-    keys and values to their codes.  Slots are distinct; tokens whose slot is outside the cache write nothing.  Positions lie in the
+    ``qkv`` may be a ``gemm.SplitK``, summed here.  Bias, per-head norms and rotation are rounded once: queries, formed in
+    fp32, to bf16, keys (fp64 in the kernel) and values to their codes.  Slots are distinct; tokens whose slot is outside the cache write nothing.  Positions lie in the
     rotary table."""
     part = None
     if not isinstance(qkv, torch.Tensor):
