@@ -11,7 +11,7 @@
 //
 // Both are bound by memory where they are large.  32 heads on 8 of 128: 4096 tokens written 20.8 us, 4.5 TB/s read and written (a copy
 // of 2 GiB 4.87), 8192 40.0, 4.7; 32768 rows read back 40 us, 5.0 TB/s.  Few tokens are a launch and a chain of two loads: 32 written 4.4 us,
-// 200 read 3.6.  Four heads a thread share a token's angles, which are as many bytes as a head and a half: 4096 tokens 21.8 -> 20.4.
+// 200 read 3.6.  Four heads a thread share a token's angles, which are as many bytes as two heads: 4096 tokens 21.8 -> 20.4.
 #include "eia_quant.h"
 
 namespace {
