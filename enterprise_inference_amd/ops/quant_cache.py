@@ -532,6 +532,8 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
         raise ValueError("quant_prefill: plan of other chunks")
     if plan.longest > block_tables.shape[1] * cache.block_size:
         raise ValueError("quant_prefill: tables shorter than the sequences")
+    if plan.longest > 0 and cache.pages == 0:       # (tiles are the plan's: the kernel would look for them)
+        raise ValueError("quant_prefill: a cache without pages holds no tokens")
     if not hip:
         at, rows = 0, []
         for s, (m, L) in enumerate(zip(plan.q_lens, plan.kv_lens)):

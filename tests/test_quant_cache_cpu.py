@@ -247,3 +247,14 @@ def test_what_is_refused():
             Q.quant_decode(q, c, bt, lens, 0.1, **kw)
         with pytest.raises(ValueError):
             Q.quant_prefill_plan([1], [5], 4, 2, 64, "cpu", **kw)
+
+
+@pytest.mark.parametrize("n", [2, 90])
+def test_a_cache_without_pages_holds_no_tokens(n):
+    """Tables that are wide enough, of a pool that is empty: chunks of few rows and of blocks."""
+    c = Q.QuantKVCache.allocate(0, 2, 16, 64)
+    q, bt, lens = torch.zeros(n, 4, 64), torch.zeros(1, 8, dtype=torch.int32), torch.full((1,), 100, dtype=torch.int32)
+    cu = torch.tensor([0, n], dtype=torch.int32)
+    with pytest.raises(ValueError, match="without pages"):
+        Q.quant_prefill(q, c, bt, lens, cu, Q.quant_prefill_plan([n], [100], 4, 2, 64, "cpu"), 0.1)
+    assert not Q.quant_prefill(q, c, bt, lens * 0, cu, Q.quant_prefill_plan([n], [0], 4, 2, 64, "cpu"), 0.1).any()
