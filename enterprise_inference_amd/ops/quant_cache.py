@@ -215,12 +215,12 @@ def rope_qkv_quant(qkv, positions: Optional[torch.Tensor], rotary, slot_mapping:
         raise ValueError("rope_qkv_quant: qkv width, cache layout")
     if (q_norm_w is None) != (k_norm_w is None):
         raise ValueError("rope_qkv_quant: norms of queries and keys together")
-    if not (slot_mapping.dtype is torch.int32 and slot_mapping.numel() >= T and slot_mapping.stride(-1) == 1):
+    if not (slot_mapping.dtype is torch.int32 and slot_mapping.numel() >= T and slot_mapping.is_contiguous()):
         raise ValueError("rope_qkv_quant: slot_mapping int32[T]")
     table, neox = None, True
     if rotary is not None:
         table, neox = rotary.cos_sin, rotary.is_neox
-        if not (positions is not None and positions.dtype is torch.int32 and positions.numel() >= T and positions.stride(-1) == 1):
+        if not (positions is not None and positions.dtype is torch.int32 and positions.numel() >= T and positions.is_contiguous()):
             raise ValueError("rope_qkv_quant: positions int32[T]")
         if not (table.shape[0] > 0 and table.shape[1] == head_dim and table.dtype is torch.float32 and table.is_contiguous()):
             raise ValueError("rope_qkv_quant: cos | sin fp32 [positions, D]")
@@ -287,7 +287,7 @@ def _check_attention(name, q, cache, block_tables, seq_lens, n, scale, window, c
     device = cache.device
     if not (q.device == device and block_tables.device == device and seq_lens.device == device):
         raise ValueError(f"{name}: one device")
-    if not (block_tables.stride(1) == 1 and seq_lens.stride(-1) == 1):
+    if not (block_tables.stride(1) == 1 and seq_lens.is_contiguous()):
         raise ValueError(f"{name}: contiguous metadata")
     return True, T, Hq
 
@@ -528,7 +528,7 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
     D = cache.head_dim
     if not (plan.num_heads == Hq and plan.num_kv_heads == cache.num_kv_heads and plan.head_dim == D):
         raise ValueError("quant_prefill: plan of other heads")
-    if not (plan.tokens == T and cu_q.numel() >= n + 1 and cu_q.dtype is torch.int32 and cu_q.stride(-1) == 1):
+    if not (plan.tokens == T and cu_q.numel() >= n + 1 and cu_q.dtype is torch.int32 and cu_q.is_contiguous()):
         raise ValueError("quant_prefill: plan of other chunks")
     if plan.longest > block_tables.shape[1] * cache.block_size:
         raise ValueError("quant_prefill: tables shorter than the sequences")

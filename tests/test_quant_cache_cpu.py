@@ -258,3 +258,20 @@ def test_a_cache_without_pages_holds_no_tokens(n):
     with pytest.raises(ValueError, match="without pages"):
         Q.quant_prefill(q, c, bt, lens, cu, Q.quant_prefill_plan([n], [100], 4, 2, 64, "cpu"), 0.1)
     assert not Q.quant_prefill(q, c, bt, lens * 0, cu, Q.quant_prefill_plan([n], [0], 4, 2, 64, "cpu"), 0.1).any()
+
+
+def test_columns_of_wider_metadata_are_refused():
+    """[n, 1] of [n, 2]: the last dimension's stride is 1, and the rows are not neighbours."""
+    c = Q.QuantKVCache.allocate(2, 2, 16, 64)
+    column = torch.zeros(4, 2, dtype=torch.int32)[:, :1]
+    assert column.stride(-1) == 1 and not column.is_contiguous()
+    rot, slots = RotaryCache(64, 10, 10000.0, None, torch.device("cpu")), torch.arange(3, dtype=torch.int32)
+    for kw in (dict(slot_mapping=column), dict(positions=column)):
+        args = dict(qkv=torch.zeros(3, 8 * 64), positions=slots, rotary=rot, slot_mapping=slots, cache=c, num_heads=4, num_kv_heads=2, head_dim=64)
+        Q.rope_qkv_quant(**args)
+        with pytest.raises(ValueError):
+            Q.rope_qkv_quant(**(args | kw))
+    q, bt, lens = torch.zeros(3, 4, 64), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    plan = Q.quant_prefill_plan([1, 1, 1], [1, 1, 1], 4, 2, 64, "cpu")
+    with pytest.raises(ValueError):
+        Q.quant_prefill(q, c, bt, lens, column, plan, 0.1)

@@ -642,3 +642,15 @@ def test_more_rows_and_heads_than_run_at_a_time(H, hk, D, bs, B):
     for s in (1, 3, B - 1):
         a = int(cu[s])
         C.check_attention(got[a:a + 2].cpu(), *_dense64(q2[a:a + 2], parts, bt[s], lens[s], 2))
+
+
+def test_lengths_that_are_a_column_are_refused():
+    """[n, 1] of [n, 2]: the last dimension's stride is 1, and the rows are not neighbours."""
+    Q = _q()
+    cache = Q.QuantKVCache.allocate(2, 1, 64, 128, "cuda")
+    q, bt, column = torch.zeros(2, 4, 128, dtype=BF, device="cuda"), _i32([[0], [1]]), _i32([[3, 0], [3, 0]])[:, :1]
+    plan = Q.quant_prefill_plan([1, 1], [3, 3], 4, 1, 128, "cuda")
+    with pytest.raises(ValueError):
+        Q.quant_decode(q, cache, bt, column, 0.1)
+    with pytest.raises(ValueError):
+        Q.quant_prefill(q, cache, bt, column, _i32([0, 1, 2]), plan, 0.1)
