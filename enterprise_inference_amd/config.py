@@ -321,6 +321,28 @@ class ParallelConfig:
         return self.tensor_parallel_size * self.pipeline_parallel_size
 
 
+def _class_attr(model: ModelConfig, name: str) -> bool:
+    from .models import get_model_class
+    try:
+        return bool(getattr(get_model_class(model.architecture), name, False))
+    except ValueError:
+        return False
+
+
+def quant_cache_refusal(model: ModelConfig, tensor_parallel_size: int = 1) -> Optional[str]:
+    """Why this model cannot be served from the 8-bit KV cache (ops/quant_cache.py); None: it can."""
+    if _class_attr(model, "allocate_cache"):
+        return ("the 8-bit KV cache is for models with the common key/value cache, not for those that lay out "
+                "their own")
+    if model.head_dim not in (64, 128, 256):
+        return f"the 8-bit KV cache takes heads of 64, 128 or 256, not {model.head_dim}"
+    group = model.num_attention_heads // tensor_parallel_size // max(1, model.num_key_value_heads // tensor_parallel_size)
+    most = 16 if model.head_dim == 256 else 32
+    if group > most:
+        return f"the 8-bit KV cache takes {most} query heads a KV head of {model.head_dim}, not {group}"
+    return None
+
+
 @dataclasses.dataclass
 class EngineConfig:
     model: ModelConfig
@@ -358,18 +380,9 @@ class EngineConfig:
         if self.cache.cache_dtype is None:
             self.cache.cache_dtype = self.dtype
         if self.cache.cache_dtype == torch.float8_e4m3fn:
-            if self._model_attr("allocate_cache"):
-                raise ValueError("the 8-bit KV cache is for models with the common key/value cache, not "
-                                 "for those that lay out their own")
-            if self.model.head_dim not in (64, 128, 256):
-                raise ValueError(f"the 8-bit KV cache takes heads of 64, 128 or 256, not {self.model.head_dim}")
-            if self.cache.block_size % 16:
-                raise ValueError(f"the 8-bit KV cache takes blocks of a multiple of 16 tokens, not {self.cache.block_size}")
-            tp = self.parallel.tensor_parallel_size
-            group = self.model.num_attention_heads // tp // max(1, self.model.num_key_value_heads // tp)
-            most = 16 if self.model.head_dim == 256 else 32
-            if group > most:
-                raise ValueError(f"the 8-bit KV cache takes {most} query heads a KV head of {self.model.head_dim}, not {group}")
+            why = quant_cache_refusal(self.model, self.parallel.tensor_parallel_size)
+            if why:
+                raise ValueError(why)
         if self._model_attr("needs_state_slots") and not self.cache.num_state_slots:
             self.cache.num_state_slots = self.scheduler.max_num_seqs
         if self.scheduler.max_model_len > self.model.max_position_embeddings and \
@@ -380,11 +393,7 @@ class EngineConfig:
             self.scheduler.max_num_batched_tokens = self.scheduler.max_num_seqs
 
     def _model_attr(self, name: str) -> bool:
-        from .models import get_model_class
-        try:
-            return bool(getattr(get_model_class(self.model.architecture), name, False))
-        except ValueError:
-            return False
+        return _class_attr(self.model, name)
 
     def _model_has_fp32_kernels(self) -> bool:
         return self._model_attr("supports_float32")

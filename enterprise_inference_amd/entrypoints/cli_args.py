@@ -134,7 +134,8 @@ def engine_config_from_args(args: argparse.Namespace):
     """Build an EngineConfig from parsed flags + the reference's env knobs."""
     import torch
 
-    from ..config import (CacheConfig, EngineConfig, ParallelConfig, SchedulerConfig, parse_dtype)
+    from ..config import (CacheConfig, EngineConfig, ParallelConfig, SchedulerConfig, parse_dtype,
+                          quant_cache_refusal)
     from ..models.loader import resolve_model_config
 
     for k in os.environ:
@@ -160,8 +161,16 @@ def engine_config_from_args(args: argparse.Namespace):
         decode_bs_bucket_step=int(os.environ.get("VLLM_DECODE_BS_BUCKET_STEP", 8)),
         delayed_sampling=_truthy(os.environ.get("VLLM_DELAYED_SAMPLING", "true")))
     kvd = (args.kv_cache_dtype or "auto").lower()
-    cache_dtype = torch.float8_e4m3fn if kvd == "fp8_per_token_head" else None
-    if cache_dtype is None and kvd not in ("auto", "bfloat16", "bf16", "float16", "fp16", "half", "float32"):
+    cache_dtype = None
+    if kvd == "fp8_per_token_head":
+        # a model that cannot have the 8-bit cache is served all the same, as with the other names
+        why = quant_cache_refusal(mcfg, args.tensor_parallel_size)
+        if why:
+            logger.warning("--kv-cache-dtype %s: %s; the KV cache stays in the model dtype (%s)",
+                           kvd, why, dtype)
+        else:
+            cache_dtype = torch.float8_e4m3fn
+    elif kvd not in ("auto", "bfloat16", "bf16", "float16", "fp16", "half", "float32"):
         # fp8 KV with one scale per tensor (vLLM --kv-cache-dtype fp8*) is not implemented: the 8-bit
         # cache keeps a scale per token and kv head.  Keep serving in the model dtype, loudly.
         logger.warning("--kv-cache-dtype %s is not supported; the KV cache stays in the model "

@@ -87,3 +87,22 @@ def test_command_line(tmp_path):
     cfg = engine_config_from_args(parse_args(base + ["--kv-cache-dtype", "fp8_per_token_head"]))
     assert cfg.cache.cache_dtype == torch.float8_e4m3fn
     assert engine_config_from_args(parse_args(base)).cache.cache_dtype == torch.float32
+
+
+@pytest.mark.parametrize("change,flags,why", [(dict(head_dim=32), [], "heads of 64"), (dict(num_attention_heads=40, num_key_value_heads=1), [], "query heads"),
+                                              (dict(num_attention_heads=72, num_key_value_heads=4), ["--tensor-parallel-size", "2"], None),
+                                              (dict(num_attention_heads=72, num_key_value_heads=2), ["--tensor-parallel-size", "2"], "query heads"),
+                                              (dict(architectures=["Sekolorn"]), [], "lay out their own")])
+def test_command_line_of_models_without_it(tmp_path, caplog, change, flags, why):
+    """They start as with the other names, in the model's type, and say why."""
+    import json
+
+    from enterprise_inference_amd.entrypoints.cli_args import engine_config_from_args, parse_args
+    (tmp_path / "config.json").write_text(json.dumps(_config("LlamaForCausalLM") | change))
+    base = ["--model", str(tmp_path), "--device", "cpu", "--load-format", "dummy", "--kv-cache-dtype", "fp8_per_token_head"]
+    with caplog.at_level("WARNING"):
+        cfg = engine_config_from_args(parse_args(base + flags))
+    if why is None:
+        assert cfg.cache.cache_dtype == torch.float8_e4m3fn and not caplog.text
+    else:
+        assert cfg.cache.cache_dtype == torch.float32 and why in caplog.text and "fp8_per_token_head" in caplog.text
