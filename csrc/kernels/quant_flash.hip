@@ -95,9 +95,8 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
   constexpr int NT = Shape<D>::THREADS, KS = Shape<D>::KS, VS = Shape<D>::VS, NV = Shape<D>::NV;
   constexpr bool TURNS = Shape<D>::TURNS;
   constexpr int PIECES = 4 * D;                            // 16-byte pieces of a tile's keys, and of its values
-  constexpr bool SHARED = PIECES < NT;                     // half the threads take keys, half values
-  constexpr int NP = SHARED ? 1 : PIECES / NT;
-  static_assert(!SHARED || 2 * PIECES == NT, "");
+  constexpr int NP = PIECES / NT;
+  static_assert(PIECES % NT == 0, "");
   __shared__ __align__(16) bf16_t lds[Shape<D>::LDS];
   bf16_t* const vlds = lds + 2 * FK * KS;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, h = lane >> 5;
@@ -125,8 +124,7 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
 
   const int* bt = a.tables + (long)it.seq * a.bt_stride;
   const int last = max(L - 1, 0) / QUANT_GROUP;
-  const bool keys_here = !SHARED || tid < PIECES, values_here = !SHARED || tid >= PIECES;
-  auto piece = [&](int i) { return SHARED ? tid % PIECES : tid + NT * i; };
+  auto piece = [&](int i) { return tid + NT * i; };
   // a wave's pieces of keys and of values lie in one group of 16 tokens, the same for both
   int page[NP], off[NP];
   auto look = [&](int tile) {
@@ -144,15 +142,11 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int pg = quant_page(__builtin_amdgcn_readfirstlane(page[i]), a.top), id = piece(i);
-      if (keys_here) {
-        const int r = id / (D / 16) % QUANT_GROUP;
-        kst[i] = *reinterpret_cast<const uint4*>(cache.key(pg, kvh, off[i] + r, D) + 16 * (id % (D / 16)));
-        ksc[i] = *cache.kscale(pg, kvh, off[i] + r);
-      }
-      if (values_here) {
-        vst[i] = *reinterpret_cast<const uint4*>(cache.values(pg, kvh, off[i], D) + 16 * (id % D));
-        vsc[i] = *reinterpret_cast<const uint4*>(cache.vscale(pg, kvh, off[i]));
-      }
+      const int r = id / (D / 16) % QUANT_GROUP;
+      kst[i] = *reinterpret_cast<const uint4*>(cache.key(pg, kvh, off[i] + r, D) + 16 * (id % (D / 16)));
+      ksc[i] = *cache.kscale(pg, kvh, off[i] + r);
+      vst[i] = *reinterpret_cast<const uint4*>(cache.values(pg, kvh, off[i], D) + 16 * (id % D));
+      vsc[i] = *reinterpret_cast<const uint4*>(cache.vscale(pg, kvh, off[i]));
     }
   };
   // Before the conversion: codes of keys that are no number, values past the end (whatever lies there, nothing of it is kept).
@@ -160,11 +154,11 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     const int kb = it.lo + FK * tile;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      if (keys_here && ksc[i] == QUANT_POISON) {
+      if (ksc[i] == QUANT_POISON) {
         ksc[i] = 127;
         kst[i] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
       }
-      if (values_here && kb + FK > L) {
+      if (kb + FK > L) {
         const int n = max(L - kb - QUANT_GROUP * (piece(i) / D), 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -181,24 +175,19 @@ quant_flash_kernel(Chunk a, QuantCache cache, const Item* __restrict__ items) {
     bf16_t* kl = lds + kbuf * (FK * KS);
     bf16_t* vl = vlds + vbuf * (D * VS);
     const int id = piece(i);
-    if (keys_here) {
-      bf16_t* p = kl + id / (D / 16) * KS + 16 * (id % (D / 16)) + 8 * h;
-      *reinterpret_cast<bf16x8*>(p) = quant_eight((&kst[i].x)[2 * h], (&kst[i].x)[2 * h + 1], quant_scale(ksc[i]));
-    }
-    if (values_here) {
-      bf16_t* p = vl + id % D * VS + QUANT_GROUP * (id / D) + 8 * h;
-      unsigned y[4];
+    bf16_t *kp = kl + id / (D / 16) * KS + 16 * (id % (D / 16)) + 8 * h, *vp = vl + id % D * VS + QUANT_GROUP * (id / D) + 8 * h;
+    *reinterpret_cast<bf16x8*>(kp) = quant_eight((&kst[i].x)[2 * h], (&kst[i].x)[2 * h + 1], quant_scale(ksc[i]));
+    unsigned y[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const unsigned word = (&vst[i].x)[2 * h + j], sb = __builtin_amdgcn_readfirstlane((&vsc[i].x)[2 * h + j]);
-        float s[4];
+    for (int j = 0; j < 2; ++j) {
+      const unsigned word = (&vst[i].x)[2 * h + j], sb = __builtin_amdgcn_readfirstlane((&vsc[i].x)[2 * h + j]);
+      float s[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) s[b] = quant_scale((sb >> (8 * b)) & 255u);
-        y[2 * j] = (quant_pair<false>(word, s[0]) & 0xffffu) | (quant_pair<false>(word, s[1]) & 0xffff0000u);
-        y[2 * j + 1] = (quant_pair<true>(word, s[2]) & 0xffffu) | (quant_pair<true>(word, s[3]) & 0xffff0000u);
-      }
-      *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
+      for (int b = 0; b < 4; ++b) s[b] = quant_scale((sb >> (8 * b)) & 255u);
+      y[2 * j] = (quant_pair<false>(word, s[0]) & 0xffffu) | (quant_pair<false>(word, s[1]) & 0xffff0000u);
+      y[2 * j + 1] = (quant_pair<true>(word, s[2]) & 0xffffu) | (quant_pair<true>(word, s[3]) & 0xffff0000u);
     }
+    *reinterpret_cast<uint4*>(vp) = make_uint4(y[0], y[1], y[2], y[3]);
   };
   auto stash_all = [&](int kbuf, int vbuf) {
 #pragma unroll

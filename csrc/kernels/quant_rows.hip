@@ -141,7 +141,6 @@ quant_rows_kernel(Rows r, QuantCache cache) {
   constexpr int KC = D / 64;         // 16-byte pieces of a key row a lane holds
   constexpr int DT = D / 16;
   constexpr bool AHEAD = D <= 128;   // keys are asked for a unit ahead; 256 channels: that costs the second workgroup on a CU
-  __shared__ bool there;
   __shared__ float sm[RW][16 * NC], sl[RW][16 * NC];
   __shared__ __align__(16) float so[RW][16 * NC][D + 4];      // (rows 16 bytes apart from a power of two)
   const int kvh = blockIdx.x, Hkv = cache.Hkv, G = r.Hq / Hkv;
