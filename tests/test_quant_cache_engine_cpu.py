@@ -106,3 +106,84 @@ def test_command_line_of_models_without_it(tmp_path, caplog, change, flags, why)
         assert cfg.cache.cache_dtype == torch.float8_e4m3fn and not caplog.text
     else:
         assert cfg.cache.cache_dtype == torch.float32 and why in caplog.text and "fp8_per_token_head" in caplog.text
+
+
+def _llama4(**kw):
+    """Layers with chunks of 24 tokens and layers without rotation, whose queries take a temperature behind the 8th token."""
+    return catalog.tiny_config("Llama4ForCausalLM", num_local_experts=4, num_experts_per_tok=1, intermediate_size=128, intermediate_size_mlp=256,
+                               num_hidden_layers=4, attention_chunk_size=24, no_rope_layers=[1, 0, 1, 0], use_qk_norm=True,
+                               attn_temperature_tuning=True, floor_scale=8, attn_scale=0.1, interleave_moe_layer_step=1, moe_layers=[1, 3],
+                               **{"head_dim": 64, **kw})
+
+
+def test_llama4_portions_give_the_tokens_of_whole_prompts():
+    """Prompts and answers cross borders of chunks; a step's plans are one for each of its layers' two forms."""
+    whole = _engine(_llama4(), mbt=512)
+    layers = whole.executor.runner.model.layers
+    assert [layer.self_attn.chunk_size for layer in layers] == [24, None, 24, None]
+    assert [layer.self_attn.temp_tuning for layer in layers] == [False, True, False, True]
+    first = _tokens(whole)
+    assert all(len(t) == 12 for t in first)
+    for mbt in (20, 33):
+        assert _tokens(_engine(_llama4(), mbt=mbt)) == first
+
+
+def test_llama4_layers_see_what_the_common_cache_gives():
+    """A step of prompts through one layer of each form: the outputs are those over a cache in the model's type whose rows are what the
+    8-bit cache keeps."""
+    from enterprise_inference_amd.ops import attention as A
+
+    runner = _engine(_llama4()).executor.runner
+    g = torch.Generator().manual_seed(3)
+    lens, bs = [60, 31], 16
+    T = sum(lens)
+    bt = torch.tensor([[0, 1, 2, 3], [4, 5, 0, 0]], dtype=torch.int32)
+    pos = torch.cat([torch.arange(n) for n in lens]).to(torch.int32)
+    slots = torch.cat([bt[s][torch.arange(n) // bs].long() * bs + torch.arange(n) % bs for s, n in enumerate(lens)]).to(torch.int32)
+    h = torch.randn(T, runner.hidden_size, generator=g)
+
+    def metadata():
+        return A.AttentionMetadata(num_decode=0, num_prefill_tokens=T, slot_mapping=slots, positions=pos, prefill_block_tables=bt,
+                                   prefill_seq_lens=torch.tensor(lens, dtype=torch.int32), prefill_cu_q=torch.tensor([0, 60, 91], dtype=torch.int32))
+
+    for layer in runner.model.layers[:2]:
+        att = layer.self_attn
+        hk, d = att.num_kv_heads, att.head_dim
+        cache = QuantKVCache.allocate(6, hk, bs, d)
+        got = att.forward(h, metadata(), cache)
+        from enterprise_inference_amd.ops.quant_cache import quant_read
+        k, v = (t.view(6, bs, hk, d).transpose(1, 2) for t in quant_read(cache, torch.arange(6 * bs, dtype=torch.int32), torch.float32))
+        kept = (k.contiguous(), v.transpose(2, 3).contiguous())
+        md = metadata()
+        md.slot_mapping = torch.full_like(slots, -1)         # the rows are there
+        want = att.forward(h, md, kept)
+        # fp32 on both sides; sums in another order, some 2^-20 of the outputs' size
+        assert float((got - want).abs().max()) <= 2 ** -18 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("tp,pp", [(2, 1), (1, 2)])
+def test_ranks_give_the_tokens_of_one(tmp_path, tp, pp):
+    """Ranks hold their heads' pages, stages their layers'; plans take the lengths that the ranks stage."""
+    from test_tensor_parallel_cpu import _ckpt
+
+    from enterprise_inference_amd.config import ParallelConfig
+    from enterprise_inference_amd.parallel import state
+
+    d = catalog.tiny_config("LlamaForCausalLM", head_dim=64, num_hidden_layers=3)
+    path = _ckpt(tmp_path, d)
+
+    def tokens(tp, pp):
+        eng = LLMEngine(EngineConfig(model=ModelConfig.from_hf_dict(d), model_path=path,
+                                     cache=CacheConfig(block_size=16, num_gpu_blocks=64, cache_dtype=torch.float8_e4m3fn),
+                                     scheduler=SchedulerConfig(max_num_seqs=4, max_num_batched_tokens=40, max_model_len=256),
+                                     parallel=ParallelConfig(tensor_parallel_size=tp, pipeline_parallel_size=pp), device="cpu",
+                                     dtype=torch.float32))
+        try:
+            kv = [c for c in eng.executor.runner.kv_caches if c is not None]
+            assert all(isinstance(c, QuantKVCache) and c.num_kv_heads == 2 // tp for c in kv) and (len(kv) < 3) == (pp > 1)
+            return _tokens(eng)
+        finally:
+            eng.shutdown()
+            state.destroy_distributed()
+
+    assert tokens(tp, pp) == tokens(1, 1)
