@@ -330,7 +330,13 @@ EIA_API int eia_quant_write(const void* qkv, long qkv_stride, const float* part,
 #define QW_D(D) do { if (neox) QW_N(D, true); else QW_N(D, false); } while (0)
   // Rows of more than a quarter of the last cache (256 MB) are read past the caches.  32 heads on 8 of 128, us as usual / past them: 4096
   // tokens (48 MiB) 20.4 / 21.0, 8192 46.1 / 39.3, 32768 184 / 172; 12 on 4 of 256, 8192 (80 MiB) 37.7 / 33.2; 12 of 64, 8192 (36 MiB) 15.8 /
-  // 19.0.  Fewer than 256 tokens spread a token a workgroup row: sixteen together would leave the chip empty.
+  // 19.0.
+  // Fewer than 256 tokens go a token a workgroup row, each with a head a thread; from there on sixteen tokens share a tile, which a whole group
+  // stores in 16-byte pieces and a group in part, in 1.3 us more, by bytes.  us, 32 heads on 8 of 128, a token a row / sixteen from a group's
+  // first slot on / from its sixth: 64 tokens 4.2 / 4.2 / 5.7, 128 4.5 / 4.3 / 5.8, 192 4.9 / 4.4 / 5.9, 255 5.2 / 5.7 / 6.0, 256 5.2 / 4.5 / 6.0, 384 6.6 /
+  // 4.7 / 6.3, 512 7.4 / 5.1 / 6.7; 12 of 64: 192 4.4 / 4.0 / 5.4, 384 5.5 / 4.0 / 5.5; 12 on 4 of 256: 192 5.1 / 4.8 / 5.8, 384 6.8 / 5.0 / 6.2.
+  // Heads a thread, one / two / four: 32 on 8 of 128, 512 tokens 5.5 / 5.2 / 5.1, 1024 9.1 / 7.3 / 7.3, 2048 13.9 / 13.0 / 11.0; 28 on 4 with bias and
+  // norms, 777 7.8 / 7.6 / 7.9, 2048 11.1 / 11.5 / 10.8; 12 on 4 of 256, 777 7.6 / 7.4 / 7.4.
   const bool once = (long)T * (Hq + 2 * Hkv) * D * 2 > 64l << 20;
   switch (D) {
     case 64: QW_D(64); break;

@@ -8,7 +8,8 @@
 //
 // A tile comes from memory as codes, half the bytes of bf16, and is converted once on its way into LDS: a key's scale is
 // the conversion's; values lie as sixteen tokens of a channel, whose scales differ, so each pair is converted twice and
-// the halves are put together (24 instructions for 16 values).  Both are exact; the products run as with a bf16 cache.
+// the halves are put together (24 instructions for 16 values).  Both are exact; the products run as with a bf16 cache, and as there
+// weights are rounded to bf16, the operand's type (half a step, 2^-8 of each).  Their sum is that of the rounded pairs: one instruction adds both.
 //
 // The host lays the launch out (which rows, which tiles): blocks that would be the launch's tail are cut along the keys,
 // their parts hand over fp32 sums and a second kernel puts them together.
@@ -17,8 +18,10 @@
 // the vector unit in some 2900 (exponentials, maxima, packing, conversion), LDS in 2300.  The halves of a workgroup take turns (by the
 // clock, with its reads in the way: scores and conversion 1100 to 1300, outputs 670; codes asked for 400 to 600, weights 1400), 555 -> 544 us
 // at 8192 tokens, 32 heads on 8; clocks fall from 2.2 to 2.0 GHz as the units fill.  1010 TFLOP/s of the causal half, where a plain bf16
-// product of 8192^3 reaches 1281.  256 channels: 515 TFLOP/s (4096
-// tokens, 12 heads on 4), one wave a SIMD, whose products wait for its own vector work; 64: 680 (8192, 16 on 4), exponentials.
+// product of 8192^3 reaches 1281.  256 channels: 515 TFLOP/s (4096 tokens, 12 heads on 4), one wave a SIMD, whose products wait for its own
+// vector work.  64: 680 (8192, 16 on 4), half the products for a score's seven vector instructions (scale and exponential, maximum, packing,
+// sum, a share of the conversion).  By counters the vector and matrix units work in 57 and 28 % of the cycles with 64 channels, 45 and 43 with
+// 128, 30 and 21 with 256.
 // Measured and left: 64 rows a wave 732 us; the next tile's first product beside this one's exponentials 550 for 547; fp8 products
 // with queries as two codes 527 for 542, but 4 us more in short launches and scores that lose their last bits.
 #include <algorithm>

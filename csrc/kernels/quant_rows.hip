@@ -7,7 +7,8 @@
 //   ends up with the scores of keys 16 g .. 16 g + 15 of column c, and these, register by register, are the P^T operands
 //   of two products whose V^T operand is the lane's 16 bytes of channel 16 dt + c: values[16 keys][channel][16].
 // A key's scale goes into the conversion of its row; a value's, with which it would have to be multiplied byte by byte,
-// into its weight.  Both are powers of two: exact.
+// into its weight.  Both are powers of two: exact.  The weight itself is rounded to bf16, the operand's type (half a step, 2^-8 of each, as with a
+// bf16 cache); their sum is that of the fp32 weights, which the lane holds (a rounded one would have to be unpacked, and freed of the value's scale).
 //
 // A launch streams the cache once; its keys are cut into parts so that every row block, or a few long ones, load the
 // whole chip.  All workgroups find the same cut from the sequences' lengths (plain sums of them: a few hundred numbers).
@@ -19,7 +20,11 @@
 // Four waves (RW) take every fourth unit and meet once at the end, or two every second, where there are more rows and heads than the chip holds
 // workgroups of four (what these are for, short chains, is gone then).  32 heads on 8 of 128, us with four / two: 128 rows of 65 to 130 keys 14.5 /
 // 12.3, of 250 to 500 30.6 / 27.4, of 1000 to 2000 79.2 / 72.8, 100 of 1000 to 2000 62.1 / 63.9; below that, 90 rows of 500 to 1000 33.2 /
-// 38.1, one of 28749 on 4 heads 17.9 / 22.3.  Meeting inside the kernel, the last part to arrive merging: one row 9.3 -> 9.9.
+// 38.1, one of 28749 on 4 heads 17.9 / 22.3.
+// Tables wider than the longest row (a captured step's are as wide as the model is long): workgroups without a part search the cut and leave,
+// which costs nothing to be seen; where no row is cut the merge is launched for nothing.  In a graph, tables as wide as the rows / 32768
+// tokens: one row of 4000 9.1 / 9.0 us, 65 of 250 to 500 19.3 / 19.4, 65 of 65 to 130 9.2 / 11.7, 128 of 65 to 130 11.7 / 14.7.
+// Meeting inside the kernel, the last part to arrive merging: one row 9.3 -> 9.9.
 #include <algorithm>
 #include <climits>
 

@@ -356,7 +356,8 @@ def quant_decode(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tenso
     """q [B, Hq, D], one token a sequence, the last of ``seq_lens`` [B] -> out [B, Hq, D] (``paged_decode`` for the 8-bit cache).
 
     Rows of length 0 become zeros.  Nothing is read back: lengths and tables may change under a captured graph, up to the
-    tables' width."""
+    tables' width.  The launch has room for what the width allows, and a second one to put parts together unless the width rules parts
+    out: no difference where rows are cut, 3 us where none is (csrc/kernels/quant_rows.hip)."""
     B = q.shape[0]
     hip, _, Hq = _check_attention("quant_decode", q, cache, block_tables, seq_lens, B, scale, sliding_window, chunk_size, out)
     if not hip:
@@ -417,7 +418,9 @@ def quant_prefill_plan(q_lens: Sequence[int], kv_lens: Sequence[int], num_heads:
 
     Sequences of few (query, head) rows go to the kernel that streams the cache for one block of them; the others are cut into
     blocks of rows, the long ones along the keys too where else the launch would wait for them.  The lists are uploaded behind the
-    current stream's work; a program that replays a captured ``quant_prefill`` keeps the plan."""
+    current stream's work.  ``quant_prefill`` waits for them on another stream, but a capture cannot: a program that replays a captured
+    ``quant_prefill`` keeps the plan, and captures when its upload is through (``torch.cuda.graph`` waits for the device before it begins;
+    who calls ``capture_begin`` synchronises first).  Host time: 20 to 500 us a plan, by blocks and by whether the launch is cut."""
     q_lens, kv_lens = [int(n) for n in q_lens], [int(n) for n in kv_lens]
     require(len(q_lens) == len(kv_lens) and all(n >= 0 for n in q_lens + kv_lens), "quant_prefill_plan: lengths")
     require(num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim in HEAD_DIMS, "quant_prefill_plan: heads")
@@ -522,7 +525,8 @@ def quant_prefill(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tens
                   plan: QuantPrefillPlan, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, Hq, D], chunks of new tokens at the end of their sequences (rows cu_q[s] .. cu_q[s + 1]), whose keys and values the
     cache already holds -> out [T, Hq, D] (``paged_prefill`` for the 8-bit cache).  ``plan`` holds the lengths that ``cu_q`` and
-    ``seq_lens`` hold on the device; rows that see no key become zeros."""
+    ``seq_lens`` hold on the device; rows that see no key become zeros.  In a capture the plan is one that is there
+    (``quant_prefill_plan``)."""
     n = len(plan.q_lens)
     hip, T, Hq = _check_attention("quant_prefill", q, cache, block_tables, seq_lens, n, scale, plan.sliding_window, plan.chunk_size, out)
     D = cache.head_dim
